@@ -217,7 +217,7 @@ def _testbed():
 def _workspace(s, size):
     if size and ("workspace" not in s or s["workspace"].numel() < size):
         s["workspace"] = torch.empty(size, device=s["dev"], dtype=torch.uint8)
-    return s["workspace"].data_ptr() if size else 0
+    return (s["workspace"].data_ptr() if size else 0), size
 
 
 def _run_own(s):
@@ -227,9 +227,9 @@ def _run_own(s):
     t = types[DTYPES[c["dtype"]]]
     if c["op"] == "dispatch":
         n, k, d = c["n"], c["k"], c["d"]
-        ws = _workspace(s, tb.expert_sort_workspace(n, k, c["experts"]))
-        tb.expert_sort(s["ids"].data_ptr(), n, k, c["experts"], s["offsets"].data_ptr(), s["order"].data_ptr(), s["slot"].data_ptr(), ws, stream)
-        tb.expert_dispatch(s["x"].data_ptr(), t, d, d, s["order"].data_ptr(), n, k, s["rows"].data_ptr(), d, stream)
+        ws, ws_bytes = _workspace(s, tb.expert_sort_workspace(n, k, c["experts"]))
+        tb.expert_sort(s["ids"].data_ptr(), n, k, c["experts"], s["offsets"].data_ptr(), s["order"].data_ptr(), s["slot"].data_ptr(), ws, ws_bytes, stream)
+        tb.expert_dispatch(s["x"].data_ptr(), t, d, d, s["order"].data_ptr(), s["slot"].data_ptr(), n, k, s["rows"].data_ptr(), d, stream)
         return s["offsets"], s["order"], s["slot"], s["rows"]
     if c["op"] == "combine":
         n, k, d = c["n"], c["k"], c["d"]
@@ -242,10 +242,10 @@ def _run_own(s):
         tb.expert_dispatch_backward(s["dx_rows"].data_ptr(), t, d, d, s["slot"].data_ptr(), n, k, s["y"].data_ptr(), d, stream)
         return s["drows"], s["dweights"], s["y"]
     m, n_in, n_out, e = c["m"], c["n_in"], c["n_out"], c.get("experts", 1)
-    ws = _workspace(s, tb.linear_i8_workspace(m, n_in, n_out, t, e))
+    ws, ws_bytes = _workspace(s, tb.linear_i8_workspace(m, n_in, n_out, t, e))
     tb.linear_i8(s["x"].data_ptr(), t, m, n_in, n_in, s["w"].data_ptr(), n_in, s["w_scale"].data_ptr(), n_out, s["y"].data_ptr(), t, n_out,
-                 bias=s["bias"].data_ptr() if c["bias"] else 0, relu=c["relu"], offsets=s["offsets"].data_ptr() if "experts" in c else 0, n_experts=e,
-                 workspace=ws, stream=stream)
+                 d_bias=s["bias"].data_ptr() if c["bias"] else 0, relu=c["relu"], d_offsets=s["offsets"].data_ptr() if "experts" in c else 0, n_experts=e,
+                 d_workspace=ws, workspace_bytes=ws_bytes, stream=stream)
     return s["y"]
 
 
