@@ -166,6 +166,64 @@ int sng_hashgrid_encode(sng_ctx* ctx, const float* d_coords, uint32_t stride_flo
  * degree 4 of the direction at d_coords[i * stride + dir_offset .. +2] (warped to [0,1]^3), d_out [n][16] fp16 */
 int sng_sh_encode(sng_ctx* ctx, const float* d_coords, uint32_t stride_floats, uint32_t dir_offset, uint32_t n, uint16_t* d_out, void* hip_stream);
 
+/* ---- operators for a field made of several experts (block fields of a large scene, a grid of small MLPs) -----------
+ * The encodings above give one row of features for each sample; these send every sample to the experts that hold it,
+ * run an expert's layers on its own rows, and blend the results: sort -> dispatch -> linear_i8 by expert -> combine.
+ * Device arrays in, device arrays out, enqueued on hip_stream on the context's device; nothing is allocated, kept
+ * between calls or synchronised, so a call can be captured into a graph.  A workspace belongs to the call that it is
+ * given to until that call has run on its stream: calls that may run at the same time (other streams, graphs) need one
+ * each.  Buffers of a call must not overlap.  ld_*: elements from one row to the next, at least the row's length. */
+enum { SNG_F16 = 0, SNG_BF16 = 1, SNG_F32 = 2, SNG_I8 = 3 };   /* element types */
+/* d_experts [n][k]: choice i = t * k + j sends sample t to an expert; an id outside [0, n_experts) drops the choice
+ * (a sample outside every block).  Out: d_offsets [n_experts + 1], the rows before each expert; d_slot [n][k], the row
+ * of each choice in the experts' order, -1 for a dropped one; d_order [n * k], the choice i of each row, -1 from
+ * d_offsets[n_experts] on.  An expert's rows keep the order of their choices.  n * k <= 2^28, n_experts <= 4096. */
+int sng_expert_sort_workspace(uint32_t n, uint32_t k, uint32_t n_experts, uint64_t* bytes);
+int sng_expert_sort(sng_ctx* ctx, const int32_t* d_experts, uint32_t n, uint32_t k, uint32_t n_experts, int32_t* d_offsets,
+                    int32_t* d_order, int32_t* d_slot, void* d_workspace, uint64_t workspace_bytes, void* hip_stream);
+/* d_rows[slot] = d_x[t] for every kept choice, rows of d elements of any type; other rows of d_rows stay as they are.
+ * Gradient: sng_expert_combine of the rows' gradients without weights. */
+int sng_expert_dispatch(sng_ctx* ctx, const void* d_x, int32_t dtype, uint32_t d, uint64_t ld_x, const int32_t* d_order,
+                        const int32_t* d_slot, uint32_t n, uint32_t k, void* d_rows, uint64_t ld_rows, void* hip_stream);
+/* d_y[t] = sum over t's kept choices of weight * row, in f32 in the order of j, rounded once; 0 where none is kept.
+ * d_weights f32 [n][k], NULL: ones.  SNG_F16, SNG_BF16, SNG_F32. */
+int sng_expert_combine(sng_ctx* ctx, const void* d_rows, int32_t dtype, uint32_t d, uint64_t ld_rows, const float* d_weights,
+                       const int32_t* d_slot, uint32_t n, uint32_t k, void* d_y, uint64_t ld_y, void* hip_stream);
+/* The combine's gradient: d_drows[slot] = weight * d_dy[t] (rows of no choice stay as they are), d_dweights[t][j] = the
+ * product <d_dy[t], d_rows[slot]> in f32 (0 for a dropped choice).  Either output may be NULL; d_rows is read for
+ * d_dweights only. */
+int sng_expert_combine_backward(sng_ctx* ctx, const void* d_dy, uint64_t ld_dy, const void* d_rows, uint64_t ld_rows, int32_t dtype,
+                                uint32_t d, const float* d_weights, const int32_t* d_slot, uint32_t n, uint32_t k, void* d_drows,
+                                uint64_t ld_drows, float* d_dweights, void* hip_stream);
+/* Rows to 8 bits: a = max(the row's largest |x|, 2^-100), q = round-half-even(127 x / a), scale = a / 127.  A row that
+ * holds an infinity or NaN gets q = 0 and scale = NaN.  Brings a layer's weights [n_out][n_in] (scale by output channel)
+ * and its input rows to what sng_linear_i8 takes. */
+int sng_quantize_rows_i8(sng_ctx* ctx, const void* d_x, int32_t dtype, uint32_t rows, uint32_t cols, uint64_t ld_x, int8_t* d_q,
+                         uint64_t ld_q, float* d_scale, void* hip_stream);
+/* y[r][c] = act((sum_k q[r][k] w[c][k]) * w_scale[c] * x_scale[r] + bias[c]): the sum exact in 32-bit integers, the rest
+ * f32, rounded once to y_dtype.  x_dtype SNG_I8: q = d_x with d_x_scale; else d_x is brought to 8 bits as above within
+ * the call.  d_offsets (sng_expert_sort's) gives rows [d_offsets[e], d_offsets[e + 1]) the e-th of n_experts matrices, one
+ * after the other in d_w, d_w_scale and d_bias; rows outside stay as they are in d_y.  d_offsets NULL: one matrix for all
+ * rows.  n_in <= 131071. */
+typedef struct {
+    const void* d_x;             /* [rows][ld_x] */
+    const float* d_x_scale;      /* [rows], SNG_I8 only */
+    const int8_t* d_w;           /* [n_experts][n_out][ld_w] */
+    const float* d_w_scale;      /* [n_experts][n_out] */
+    const float* d_bias;         /* [n_experts][n_out] or NULL */
+    const int32_t* d_offsets;    /* [n_experts + 1] or NULL */
+    void* d_y;                   /* [rows][ld_y] */
+    void* d_workspace;           /* sng_linear_i8_workspace bytes, aligned to 16 */
+    uint64_t workspace_bytes;
+    uint64_t ld_x, ld_w, ld_y;
+    uint32_t rows, n_in, n_out, n_experts;
+    int32_t x_dtype, y_dtype;
+    int32_t relu;                /* 1: max(., 0) */
+    int32_t reserved;
+} sng_linear_i8_args;
+int sng_linear_i8_workspace(uint32_t rows, uint32_t n_in, uint32_t n_out, int32_t x_dtype, uint32_t n_experts, uint64_t* bytes);
+int sng_linear_i8(sng_ctx* ctx, const sng_linear_i8_args* args, void* hip_stream);
+
 /* ---- virtual scene: Engine::set_virtual_world + Engine::init keys (engine.cu:21-78, 129-234) */
 int sng_load_virtual_scene(sng_ctx* ctx, const char* json_path);
 int sng_clear_virtual_scene(sng_ctx* ctx);

@@ -119,6 +119,31 @@ class sng_material(ctypes.Structure):
     ]
 
 
+class sng_linear_i8_args(ctypes.Structure):
+    _fields_ = [
+        ("d_x", ctypes.c_void_p),
+        ("d_x_scale", ctypes.c_void_p),
+        ("d_w", ctypes.c_void_p),
+        ("d_w_scale", ctypes.c_void_p),
+        ("d_bias", ctypes.c_void_p),
+        ("d_offsets", ctypes.c_void_p),
+        ("d_y", ctypes.c_void_p),
+        ("d_workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+        ("ld_x", ctypes.c_uint64),
+        ("ld_w", ctypes.c_uint64),
+        ("ld_y", ctypes.c_uint64),
+        ("rows", ctypes.c_uint32),
+        ("n_in", ctypes.c_uint32),
+        ("n_out", ctypes.c_uint32),
+        ("n_experts", ctypes.c_uint32),
+        ("x_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32),
+        ("relu", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class sng_object_info(ctypes.Structure):
     _fields_ = [
         ("n_nodes", ctypes.c_uint32),
@@ -186,6 +211,14 @@ SIGNATURES = {
     "sng_nerf_inference": (ctypes.c_int, [P, P, U32, U32, P, I32, P]),
     "sng_hashgrid_encode": (ctypes.c_int, [P, P, U32, U32, P, P]),
     "sng_sh_encode": (ctypes.c_int, [P, P, U32, U32, U32, P, P]),
+    "sng_expert_sort_workspace": (ctypes.c_int, [U32, U32, U32, ctypes.POINTER(U64)]),
+    "sng_expert_sort": (ctypes.c_int, [P, P, U32, U32, U32, P, P, P, P, U64, P]),
+    "sng_expert_dispatch": (ctypes.c_int, [P, P, I32, U32, U64, P, P, U32, U32, P, U64, P]),
+    "sng_expert_combine": (ctypes.c_int, [P, P, I32, U32, U64, P, P, U32, U32, P, U64, P]),
+    "sng_expert_combine_backward": (ctypes.c_int, [P, P, U64, P, U64, I32, U32, P, P, U32, U32, P, U64, P, P]),
+    "sng_quantize_rows_i8": (ctypes.c_int, [P, P, I32, U32, U32, U64, P, U64, P, P]),
+    "sng_linear_i8_workspace": (ctypes.c_int, [U32, U32, U32, I32, U32, ctypes.POINTER(U64)]),
+    "sng_linear_i8": (ctypes.c_int, [P, ctypes.POINTER(sng_linear_i8_args), P]),
     "sng_load_virtual_scene": (ctypes.c_int, [P, ctypes.c_char_p]),
     "sng_clear_virtual_scene": (ctypes.c_int, [P]),
     "sng_set_param": (ctypes.c_int, [P, ctypes.c_char_p, ctypes.c_double]),

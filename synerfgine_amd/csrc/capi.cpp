@@ -9,6 +9,7 @@
 // The runtime is split by subsystem (host.h lists its files); this file holds the C ABI itself, the context's
 // creation and destruction, and the small utilities the others share.
 #include "host.h"
+#include "host_operators.h"
 
 namespace sng_host {
 
@@ -257,6 +258,41 @@ int sng_sh_encode(sng_ctx* c, const float* coords, uint32_t stride, uint32_t dir
         launch_sh_encode(coords, stride, dir_offset, n, out, (hipStream_t)stream);
         HIPCHK(hipGetLastError());
     });
+}
+
+int sng_expert_sort_workspace(uint32_t n, uint32_t k, uint32_t n_experts, uint64_t* bytes) {
+    return guarded([&] {
+        if (!bytes) throw SngError(SNG_ERR_INVALID, "null argument");
+        *bytes = expert_sort_workspace(n, k, n_experts);
+    });
+}
+int sng_expert_sort(sng_ctx* c, const int32_t* experts, uint32_t n, uint32_t k, uint32_t n_experts, int32_t* offsets, int32_t* order, int32_t* slot, void* workspace,
+                    uint64_t workspace_bytes, void* stream) {
+    return guarded([&] { expert_sort(c, experts, n, k, n_experts, offsets, order, slot, workspace, workspace_bytes, (hipStream_t)stream); });
+}
+int sng_expert_dispatch(sng_ctx* c, const void* x, int32_t dtype, uint32_t d, uint64_t ld_x, const int32_t* order, const int32_t* slot, uint32_t n, uint32_t k, void* rows,
+                        uint64_t ld_rows, void* stream) {
+    return guarded([&] { expert_dispatch(c, x, dtype, d, ld_x, order, slot, n, k, rows, ld_rows, (hipStream_t)stream); });
+}
+int sng_expert_combine(sng_ctx* c, const void* rows, int32_t dtype, uint32_t d, uint64_t ld_rows, const float* weights, const int32_t* slot, uint32_t n, uint32_t k, void* y,
+                       uint64_t ld_y, void* stream) {
+    return guarded([&] { expert_combine(c, rows, dtype, d, ld_rows, weights, slot, n, k, y, ld_y, (hipStream_t)stream); });
+}
+int sng_expert_combine_backward(sng_ctx* c, const void* dy, uint64_t ld_dy, const void* rows, uint64_t ld_rows, int32_t dtype, uint32_t d, const float* weights,
+                                const int32_t* slot, uint32_t n, uint32_t k, void* drows, uint64_t ld_drows, float* dweights, void* stream) {
+    return guarded([&] { expert_combine_backward(c, dy, ld_dy, rows, ld_rows, dtype, d, weights, slot, n, k, drows, ld_drows, dweights, (hipStream_t)stream); });
+}
+int sng_quantize_rows_i8(sng_ctx* c, const void* x, int32_t dtype, uint32_t rows, uint32_t cols, uint64_t ld_x, int8_t* q, uint64_t ld_q, float* scale, void* stream) {
+    return guarded([&] { quantize_rows_i8(c, x, dtype, rows, cols, ld_x, q, ld_q, scale, (hipStream_t)stream); });
+}
+int sng_linear_i8_workspace(uint32_t rows, uint32_t n_in, uint32_t n_out, int32_t x_dtype, uint32_t n_experts, uint64_t* bytes) {
+    return guarded([&] {
+        if (!bytes) throw SngError(SNG_ERR_INVALID, "null argument");
+        *bytes = linear_i8_workspace(rows, n_in, n_out, x_dtype, n_experts);
+    });
+}
+int sng_linear_i8(sng_ctx* c, const sng_linear_i8_args* args, void* stream) {
+    return guarded([&] { linear_i8(c, args, (hipStream_t)stream); });
 }
 
 int sng_load_virtual_scene(sng_ctx* c, const char* path) { return guarded([&] { load_scene(c, path); }); }
