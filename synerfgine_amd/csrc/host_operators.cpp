@@ -145,7 +145,7 @@ void quantize_rows_i8(sng_ctx* c, const void* x, int32_t dtype, uint32_t rows, u
 uint64_t linear_i8_workspace(uint32_t rows, uint32_t n_in, uint32_t n_out, int32_t x_dtype, uint32_t n_experts) {
     check_linear(rows, n_in, n_out, n_experts);
     check_type(x_dtype, true);
-    if (x_dtype == SNG_I8) return 0;
+    if (rows == 0 || x_dtype == SNG_I8 || linear_i8_quantizes(linear_i8_kernel(rows, n_in, n_out, n_experts), rows, n_experts)) return 0;
     return rows * padded(n_in) + (uint64_t)rows * sizeof(float);
 }
 
@@ -169,16 +169,16 @@ void linear_i8(sng_ctx* c, const sng_linear_i8_args* p, hipStream_t s) {
     OnDevice on(c);
     if (a.rows == 0) return;
     LinearArgs l{};
-    l.x = (const int8_t*)a.d_x; l.ld_x = a.ld_x; l.x_scale = a.d_x_scale; l.w = a.d_w; l.ld_w = a.ld_w; l.w_scale = a.d_w_scale; l.bias = a.d_bias;
+    l.x = a.d_x; l.ld_x = a.ld_x; l.x_dtype = a.x_dtype; l.x_scale = a.d_x_scale; l.w = a.d_w; l.ld_w = a.ld_w; l.w_scale = a.d_w_scale; l.bias = a.d_bias;
     l.offsets = a.d_offsets; l.n_experts = a.n_experts; l.rows = a.rows; l.n_in = a.n_in; l.n_out = a.n_out; l.y = a.d_y; l.ld_y = a.ld_y;
     l.y_dtype = a.y_dtype; l.relu = a.relu;
-    if (a.x_dtype != SNG_I8) {
+    if (need) {
         const uint64_t ld = padded(a.n_in);
         int8_t* q = (int8_t*)a.d_workspace;
         float* scale = (float*)(q + a.rows * ld);
         launch_quantize_rows(QuantArgs{a.d_x, a.ld_x, a.x_dtype, a.rows, a.n_in, (uint32_t)ld, q, ld, scale}, s);
         HIPCHK(hipGetLastError());
-        l.x = q; l.ld_x = ld; l.x_scale = scale;
+        l.x = q; l.ld_x = ld; l.x_dtype = SNG_I8; l.x_scale = scale;
     }
     launch_linear_i8(l, s);
     HIPCHK(hipGetLastError());

@@ -74,9 +74,10 @@ struct QuantArgs {
     float* scale;            // not written for DT_I8
 };
 struct LinearArgs {
-    const int8_t* x;         // [rows][ld_x]
-    uint64_t ld_x;
-    const float* x_scale;    // [rows]
+    const void* x;           // [rows][ld_x] of x_dtype
+    uint64_t ld_x;           // elements
+    int x_dtype;
+    const float* x_scale;    // [rows], DT_I8
     const int8_t* w;         // [n_experts][n_out][ld_w]
     uint64_t ld_w;
     const float* w_scale;    // [n_experts][n_out]
@@ -87,6 +88,11 @@ struct LinearArgs {
     uint64_t ld_y;
     int y_dtype, relu;
 };
+// Which kernel: by the sizes alone, so that the workspace's size is known before the call.
+enum class LinearKernel { Rows, Few, Tile };
+LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts);
+// whether the kernel brings x to 8 bits itself (else x has to be DT_I8)
+bool linear_i8_quantizes(LinearKernel k, uint32_t rows, uint32_t n_experts);
 void launch_quantize_rows(const QuantArgs& a, hipStream_t s);
 void launch_linear_i8(const LinearArgs& a, hipStream_t s);
 
