@@ -5,6 +5,7 @@
 //
 // The sum is exact (int32; n_in <= 131071), the rest is f32 and is rounded once, to y's type.
 #include <algorithm>
+#include <type_traits>
 
 #include "operators.h"
 
@@ -278,38 +279,47 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {
 // three lanes of its row, so a store writes 64 consecutive bytes a row: 8 channels of f16 (two accumulators), 4 of f32.
 __device__ __forceinline__ uint32_t channel_of(int t, uint32_t g, bool wide) { return wide ? t * 16 + g * 4 : (t >> 1) * 32 + g * 8 + (t & 1) * 4; }
 
-// One row's 16 channels of a 64-channel block (v[4 t + i], channels as channel_of says), `left` channels from the block's first on
-__device__ __forceinline__ void store_block(const LinearArgs& a, uint32_t row, uint32_t c0, uint32_t g, const float (&v)[16], uint32_t left, bool aligned) {
-    if (a.y_dtype == DT_F32) {
-        float* y = (float*)a.y + (uint64_t)row * a.ld_y + c0;
+// 16 bytes of y: 4 f32 or 8 16-bit channels of a row from channel c on, `left` of them inside
+template <int N>
+__device__ __forceinline__ void store_piece(const LinearArgs& a, uint32_t row, uint32_t c, const float (&v)[N], uint32_t left, bool aligned) {
+    const uint64_t at = (uint64_t)row * a.ld_y + c;
+    if constexpr (N == 4) {
+        float* y = (float*)a.y + at;
+        if (aligned && left >= 4) *(vec<float, 4>*)y = vec<float, 4>{v[0], v[1], v[2], v[3]};
+        else
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint32_t c = channel_of(t, g, true);
-            if (aligned && c + 4 <= left) *(vec<float, 4>*)(y + c) = vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
-            else
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (c + i < left) y[c + i] = v[4 * t + i];
-        }
-        return;
-    }
-    uint16_t* y = (uint16_t*)a.y + (uint64_t)row * a.ld_y + c0;
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        const uint32_t c = channel_of(2 * p, g, false);
+            for (int i = 0; i < 4; ++i)
+                if ((uint32_t)i < left) y[i] = v[i];
+    } else {
+        uint16_t* y = (uint16_t*)a.y + at;
         vec<uint16_t, 8> o;
         if (a.y_dtype == DT_F16)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __builtin_bit_cast(uint16_t, (_Float16)v[8 * p + i]);
+            for (int i = 0; i < 8; ++i) o[i] = __builtin_bit_cast(uint16_t, (_Float16)v[i]);
         else
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __builtin_bit_cast(uint16_t, (__bf16)v[8 * p + i]);
-        if (aligned && c + 8 <= left) *(vec<uint16_t, 8>*)(y + c) = o;
+            for (int i = 0; i < 8; ++i) o[i] = __builtin_bit_cast(uint16_t, (__bf16)v[i]);
+        if (aligned && left >= 8) *(vec<uint16_t, 8>*)y = o;
         else
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (c + i < left) y[c + i] = o[i];
+                if ((uint32_t)i < left) y[i] = o[i];
     }
+}
+// One row's 16 channels of a 64-channel block (v[4 t + i], channels as channel_of says), `left` channels from the block's first on
+__device__ __forceinline__ void store_block(const LinearArgs& a, uint32_t row, uint32_t c0, uint32_t g, const float (&v)[16], uint32_t left, bool aligned) {
+    if (a.y_dtype == DT_F32) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint32_t c = channel_of(t, g, true);
+            store_piece(a, row, c0 + c, {v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]}, left - min(left, c), aligned);
+        }
+    } else
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t c = channel_of(2 * p, g, false);
+            store_piece(a, row, c0 + c, {v[8 * p], v[8 * p + 1], v[8 * p + 2], v[8 * p + 3], v[8 * p + 4], v[8 * p + 5], v[8 * p + 6], v[8 * p + 7]}, left - min(left, c), aligned);
+        }
 }
 __device__ __forceinline__ bool y_aligned(const LinearArgs& a) { return (((uint64_t)a.y | (a.ld_y * (a.y_dtype == DT_F32 ? 4 : 2))) & 15) == 0; }
 
@@ -602,73 +612,91 @@ __global__ __launch_bounds__(256) void linear_i8_tile_kernel(LinearArgs a) {
 }
 
 // The same product with both tiles brought straight into LDS (global_load_lds, 16 bytes a lane): no registers and no
-// instructions stand between memory and the matrix units.  Rows of 128 bytes; a lane fetches the piece of its row that
-// belongs at its place in LDS, which keeps the eight lanes of a fragment read's phase on different banks: piece ^ (r & 7)
-// for the row that is fragment row r of the reads (the channels of a fragment are not consecutive, see channel_of).  Two stages: a step's loads are on their way while the step before is multiplied, one barrier a step.
+// instructions stand between memory and the matrix units.  Steps of 128 bytes of n_in (whole cache lines), a stage of LDS
+// each, in halves: while one half is multiplied from registers the next is read from LDS.  Once a step's second half is in
+// registers its stage is free: the one barrier of the step, behind which the loads of STAGES steps ahead refill it.  Loads and
+// reads are spread between the matrix instructions: behind the barrier every wave would else queue its loads first and
+// the matrix units would wait for the queue.  A lane fetches the piece of its row that belongs at its place in LDS, which
+// keeps the lanes of a fragment read on different banks.
 // Wants n_in, both strides and both addresses in multiples of 16 bytes.
-template <int BM, int BN, bool WIDE>
-__global__ __launch_bounds__(BM * BN / 128) void linear_i8_stream_kernel(LinearArgs a, uint32_t col_tiles, uint32_t tiles) {
-    constexpr int WC = BN / 64, WAVES = BM * BN / 128 / 64, WR = WAVES / WC, XT = BM / WR / 16, BK = 128, STAGE = (BM + BN) * BK;
+__device__ const int8_t zeros16[16] __attribute__((aligned(16))) = {};
+
+// A wave holds BM / WR rows by 64 channels.
+template <int BM, int BN, int WR, int STAGES, bool WIDE>
+__global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a, uint32_t col_tiles, uint32_t tiles) {
+    constexpr int WC = BN / 64, WAVES = WR * WC, XT = BM / WR / 16, BK = 128, STAGE = (BM + BN) * BK;
     constexpr int LOADS = (BM + BN) / 8 / WAVES;   // each brings 8 rows of 128 bytes
-    __shared__ __align__(16) int8_t lds[2 * STAGE];
+    __shared__ __align__(16) int8_t lds[STAGES * STAGE];
     // workgroups go round the 8 dies one by one: each die gets a run of neighbouring tiles, in columns of 4 row tiles, so
     // that its cache sees the same rows and channels again
     const uint32_t per = (tiles + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (id >= tiles) return;
     const uint32_t row_tiles = tiles / col_tiles, group = id / (4 * col_tiles), in = id - group * 4 * col_tiles, high = min(4u, row_tiles - group * 4);
-    const RowTile tile = row_tile(a, group * 4 + in % high, BM == 256 ? 8 : 7);
+    const RowTile tile = row_tile(a, group * 4 + in % high, BM == 256 ? 8 : BM == 128 ? 7 : 6);
     if (tile.begin >= tile.end) return;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15, n0 = in / high * BN;
     const uint32_t wm = wave / WC * (BM / WR), wn = wave % WC * 64;
-    // this lane's loads: tile rows wave * LOADS * 8 + i * 8 + lane / 8
+    // this lane's loads: tile rows (wave + i * WAVES) * 8 + lane / 8.  Place p of fragment row r holds piece p ^ (r / 2 & 7):
+    // the 16 lanes that LDS serves at a time (0-3, 12-15, 20-23, 24-27 and so on) then cover its 64 banks
+    static_assert(WAVES % 4 == 0, "the bits of a row that its place depends on are the same for all of a lane's loads");
+    const uint32_t row8 = lane >> 3, piece_x = ((lane & 7) ^ (row8 >> 1 | (wave & 1) << 2)) * 16;
+    const uint32_t piece_w = WIDE ? piece_x : ((lane & 7) ^ ((row8 >> 1 & 1) | (wave & 3) << 1)) * 16;
     const int8_t* from[LOADS];
-    const bool of_w = wave * LOADS * 8 >= BM;
-    uint32_t piece[2];   // of even and odd loads
-#pragma unroll
-    for (int i = 0; i < 2; ++i) piece[i] = ((lane & 7) ^ (of_w && !WIDE ? ((lane >> 3) & 3) | (i << 2) : lane >> 3)) * 16;
-    static_assert(LOADS % 2 == 0 && BM % (LOADS * 8) == 0, "a wave's loads are all of x or all of w");
+    uint32_t piece[LOADS];   // (the compiler keeps one of each kind)
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const uint32_t row = (wave * LOADS + i) * 8 + (lane >> 3);
-        if (row < BM) from[i] = (const int8_t*)a.x + (uint64_t)min(tile.begin + row, tile.end - 1) * a.ld_x;
-        else from[i] = a.w + ((uint64_t)tile.expert * a.n_out + min(n0 + row - BM, a.n_out - 1)) * a.ld_w;
+        const uint32_t row = (wave + i * WAVES) * 8 + row8;   // (8 rows are all of x or all of w)
+        const bool of_x = (wave + i * WAVES) * 8 < BM;
+        piece[i] = of_x ? piece_x : piece_w;
+        if (of_x) from[i] = (const int8_t*)a.x + (uint64_t)min(tile.begin + row, tile.end - 1) * a.ld_x + piece_x;
+        else from[i] = a.w + ((uint64_t)tile.expert * a.n_out + min(n0 + row - BM, a.n_out - 1)) * a.ld_w + piece_w;
     }
-    const auto load = [&](uint32_t k0, int stage) {
-        // (past the end: anything, the rows' fragments are cleared there)
-        const uint32_t k[2] = {k0 + piece[0] < a.n_in ? k0 + piece[0] : 0, k0 + piece[1] < a.n_in ? k0 + piece[1] : 0};
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from[i] + k[i & 1]),
-                                             (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (wave * LOADS + i) * 1024), 16, 0, 0);
+    // (pieces past the end are zeros; steps past the last are loaded too, so that the number of loads on their way is the
+    // same in every step)
+    const auto load = [&](uint32_t step, int i) {
+        const int8_t* p = step * BK + piece[i] < a.n_in ? from[i] + step * BK : zeros16;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                         (__attribute__((address_space(3))) void*)(lds + step % STAGES * STAGE + (wave + i * WAVES) * 1024), 16, 0, 0);
     };
-    i4 acc[4][XT];
+    i4 acc[4][XT] = {};
+    const uint32_t key = r >> 1;
+    const uint32_t at_x = (wm + r) * BK + (g ^ key) * 16, at_w = (BM + wn + channel_of(0, r >> 2, WIDE) + (r & 3)) * BK + (g ^ key) * 16;
+    struct Fragments { i4 x[XT], w[4]; };   // of 64 bytes
+    const auto read_w = [&](uint32_t step, int h, Fragments& f, int t) { f.w[t] = *(const i4*)(lds + step % STAGES * STAGE + (at_w ^ (h * 64)) + channel_of(t, 0, WIDE) * BK); };
+    const auto read_x = [&](uint32_t step, int h, Fragments& f, int u) { f.x[u] = *(const i4*)(lds + step % STAGES * STAGE + (at_x ^ (h * 64)) + u * 16 * BK); };
+    // all but the newest `left` of this wave's loads have come, its own reads of LDS too, and the same holds for every wave
+    const auto meet = [&](auto left) { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(left)::value) : "memory"); };
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int s = 0; s < STAGES; ++s)
 #pragma unroll
-        for (int u = 0; u < XT; ++u) acc[t][u] = i4{0, 0, 0, 0};
-    const uint32_t at_x = (wm + r) * BK + ((g ^ (r & 7)) * 16), at_w = (BM + wn + channel_of(0, r >> 2, WIDE) + (r & 3)) * BK + ((g ^ (r & 7)) * 16);
-    load(0, 0);
-    int stage = 0;
-    for (uint32_t k0 = 0; k0 < a.n_in; k0 += BK, stage ^= 1) {
-        __syncthreads();   // this step's loads are there, and nobody reads the other stage any more
-        if (k0 + BK < a.n_in) load(k0 + BK, stage ^ 1);
-        const int8_t* tile_lds = lds + stage * STAGE;
+        for (int i = 0; i < LOADS; ++i) load(s, i);
+    Fragments f[2];
+    meet(std::integral_constant<int, (STAGES - 1) * LOADS>{});
+#pragma unroll
+    for (int t = 0; t < 4; ++t) read_w(0, 0, f[0], t);
+#pragma unroll
+    for (int u = 0; u < XT; ++u) read_x(0, 0, f[0], u);
+    const uint32_t steps = (a.n_in + BK - 1) / BK;
+    for (uint32_t step = 0; step < steps; ++step) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            i4 fx[XT], fw[4];
+            if (h == 1) meet(std::integral_constant<int, (STAGES - 2) * LOADS>{});   // this step's stage has been read, the next step's has come
+            // XT pieces: four matrix instructions, a row fragment, and their share of the channel fragments and of the loads
 #pragma unroll
-            for (int t = 0; t < 4; ++t) fw[t] = *(const i4*)(tile_lds + (at_w ^ (h * 64)) + channel_of(t, 0, WIDE) * BK);
+            for (int u = 0; u < XT; ++u) {
 #pragma unroll
-            for (int u = 0; u < XT; ++u) fx[u] = *(const i4*)(tile_lds + (at_x ^ (h * 64)) + u * 16 * BK);
-            if (k0 + BK > a.n_in && k0 + h * 64 + g * 16 >= a.n_in)
+                for (int q = u * 4 / XT; q < (u + 1) * 4 / XT; ++q) read_w(step + h, h ^ 1, f[h ^ 1], q);
+                read_x(step + h, h ^ 1, f[h ^ 1], u);
+                if (h == 1)
 #pragma unroll
-                for (int u = 0; u < XT; ++u) fx[u] = i4{0, 0, 0, 0};
+                    for (int q = u * LOADS / XT; q < (u + 1) * LOADS / XT; ++q) load(step + STAGES, q);
 #pragma unroll
-            for (int u = 0; u < XT; ++u)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[t], fx[u], acc[t][u], 0, 0, 0);
+                for (int t = 0; t < 4; ++t) acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[h].w[t], f[h].x[u], acc[t][u], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load may reach LDS after the workgroup has left it
     const uint32_t c0 = n0 + wn;
     if (c0 >= a.n_out) return;
     const bool aligned = y_aligned(a);
@@ -700,11 +728,11 @@ static void linear(const LinearArgs& a, hipStream_t s) {
     linear_i8_tile_kernel<T, 128, 128><<<dim3(row_tiles(a, 7), (a.n_out + 127) / 128), 256, 0, s>>>(a);
 }
 
-template <int BM, int BN>
+template <int BM, int BN, int WR, int STAGES>
 static void linear_stream(const LinearArgs& a, hipStream_t s) {
-    const uint32_t cols = (a.n_out + BN - 1) / BN, tiles = row_tiles(a, BM == 256 ? 8 : 7) * cols, grid = (tiles + 7) / 8 * 8;
-    if (a.y_dtype == DT_F32) linear_i8_stream_kernel<BM, BN, true><<<grid, BM * BN / 128, 0, s>>>(a, cols, tiles);
-    else linear_i8_stream_kernel<BM, BN, false><<<grid, BM * BN / 128, 0, s>>>(a, cols, tiles);
+    const uint32_t cols = (a.n_out + BN - 1) / BN, tiles = row_tiles(a, BM == 256 ? 8 : BM == 128 ? 7 : 6) * cols, grid = (tiles + 7) / 8 * 8;
+    if (a.y_dtype == DT_F32) linear_i8_stream_kernel<BM, BN, WR, STAGES, true><<<grid, BN * WR, 0, s>>>(a, cols, tiles);
+    else linear_i8_stream_kernel<BM, BN, WR, STAGES, false><<<grid, BN * WR, 0, s>>>(a, cols, tiles);
 }
 
 LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
@@ -730,8 +758,11 @@ void launch_linear_i8(const LinearArgs& a, hipStream_t s) {
         case LinearKernel::Tile: break;
     }
     if (((uint64_t)a.x | a.ld_x | (uint64_t)a.w | a.ld_w | a.n_in) % 16 == 0) {
-        if ((uint64_t)(a.rows / 256) * (a.n_out / 256) >= 192) linear_stream<256, 256>(a, s);
-        else linear_stream<128, 128>(a, s);
+        // the largest tile that still gives most of the 256 CUs one: 256 x 256 reads each operand least often
+        const uint64_t cells = (uint64_t)a.rows * a.n_out;
+        if (cells >= 192ull * 256 * 256) linear_stream<256, 256, 2, 2>(a, s);
+        else if (cells >= 192ull * 128 * 128) linear_stream<128, 128, 2, 2>(a, s);
+        else linear_stream<64, 128, 2, 4>(a, s);
         return;
     }
     if (a.y_dtype == DT_F16) linear<_Float16>(a, s);
