@@ -1,0 +1,168 @@
+// linear_i8_rows.hip -- the 8-bit linear layer for short rows (linear_i8.hip describes the layer)
+#include "linear_i8.h"
+
+namespace sng {
+
+// n_in <= 256: a row is at most 4 fragments of 64 bytes, so a wave loads 16 rows, finds their scales, brings them to 8 bits
+// and multiplies them without leaving its registers: x is read once and y written once, the floor of a layer this small.
+// A lane holds the 16 consecutive values of one row that the matrix instruction wants of it; the four lanes of a row share
+// their maximum with two shuffles.  The weights of up to 256 channels lie in LDS in fragment order (one linear
+// ds_read_b128 a fragment, no bank conflicts), staged once for the workgroup's rows, which belong to one expert.
+// x of type DT; KC fragments of 64 a row; NB blocks of 64 channels.  YT: y's type where every piece is a whole one (n_in in
+// 16s, n_out in 8s, y aligned to 16 bytes); -1: any sizes and places, at more registers and so fewer waves.  What hides the
+// memory's latency here is waves: under 64 registers 8 a SIMD, and small workgroups.
+template <int DT, int YT, int KC, int NB>
+__global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint32_t shift) {
+    constexpr int XB = bytes_of(DT);
+    constexpr bool WHOLE = YT >= 0;
+    __shared__ i4 lw[NB * 4 * KC * 64];
+    __shared__ __align__(16) float lscale[NB * 64], lbias[NB * 64];
+    const RowTile tile = row_tile(a, blockIdx.x, shift);
+    if (tile.begin >= tile.end) return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n0 = blockIdx.y * (NB * 64), n = a.n_in;
+    const bool wide = WHOLE ? YT == DT_F32 : a.y_dtype == DT_F32, aligned = WHOLE || y_aligned(a);
+    const auto fetch = [&](uint32_t r0, Raw<DT, 16> (&raw)[KC]) {
+        const char* row = (const char*)a.x + (uint64_t)min(r0 + (lane & 15), tile.end - 1) * a.ld_x * XB;
+        if (!WHOLE && n < 16)
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) raw[kc] = load_short_row<DT>(row, kc * 64 + g * 16, n);
+        else
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) raw[kc] = load_row16<DT>(row, kc * 64 + g * 16, n);
+    };
+    Raw<DT, 16> raw[KC];
+    uint32_t r0 = tile.begin + wave * 16;
+    if (r0 < tile.end) fetch(r0, raw);
+    {
+        const int8_t* __restrict__ w = (const int8_t*)a.w + (uint64_t)tile.expert * a.n_out * a.ld_w;
+        const auto w_row = [&](int i) {   // the channel and place in it of fragment lane i * 256 + tid
+            const uint32_t f = i * 256 + threadIdx.x, t = (f >> 6) / KC & 3, nb = (f >> 6) / (4 * KC);
+            return (const char*)w + (uint64_t)min(n0 + nb * 64 + channel_of(t, (f >> 2) & 3, wide) + (f & 3), a.n_out - 1) * a.ld_w;
+        };
+        const auto w_k = [&](int i) { return ((i * 256 + threadIdx.x) >> 6) % KC * 64 + ((threadIdx.x & 63) >> 4) * 16; };
+#pragma unroll
+        for (int i0 = 0; i0 < NB * KC; i0 += 4) {   // (up to four loads at a time: registers)
+            constexpr int I = NB * KC < 4 ? NB * KC : 4;
+            Raw<DT_I8, 16> fw[I];
+            if (!WHOLE && n < 16)
+#pragma unroll
+                for (int i = 0; i < I; ++i) fw[i] = load_short_row<DT_I8>(w_row(i0 + i), w_k(i0 + i), n);
+            else {
+#pragma unroll
+                for (int i = 0; i < I; ++i) fw[i] = load_row16<DT_I8>(w_row(i0 + i), w_k(i0 + i), n);
+                if (n != KC * 64)
+#pragma unroll
+                    for (int i = 0; i < I; ++i) keep_inside<DT_I8, WHOLE>(fw[i], w_k(i0 + i), n);
+            }
+#pragma unroll
+            for (int i = 0; i < I; ++i) lw[(i0 + i) * 256 + threadIdx.x] = as_fragment(fw[i]);   // (channels past the last: multiplied, not stored)
+        }
+        if (threadIdx.x < NB * 64) {
+            const uint32_t c = n0 + threadIdx.x;
+            const uint64_t at = (uint64_t)tile.expert * a.n_out + c;
+            lscale[threadIdx.x] = c < a.n_out ? a.w_scale[at] : 0.0f;
+            lbias[threadIdx.x] = c < a.n_out && a.bias ? a.bias[at] : 0.0f;
+        }
+    }
+    __syncthreads();
+    const float low = lowest(a);
+    for (; r0 < tile.end; r0 += 64) {
+        asm volatile("" ::: "memory");   // (else the scales are kept over the loop, in the registers of several waves)
+        const uint32_t row = r0 + (lane & 15);
+        i4 q[KC];
+        float scale;
+        if (n != KC * 64 && (WHOLE || n >= 16))
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) keep_inside<DT, WHOLE>(raw[kc], kc * 64 + g * 16, n);
+        if constexpr (DT == DT_I8) {
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) q[kc] = as_fragment(raw[kc]);
+            scale = a.x_scale[min(row, tile.end - 1)];
+        } else {
+            uint32_t top = 0;
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) top = max(top, top_bits(raw[kc]));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+            const RowScale rs = row_scale(top);
+            scale = rs.scale;
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) q[kc] = quantize_n(raw[kc], rs);
+        }
+        if (r0 + 64 < tile.end) fetch(r0 + 64, raw);   // before the stores: a wait for loads is one for the stores before them too
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const uint32_t c0 = n0 + nb * 64;
+            if (c0 >= a.n_out) break;
+            const uint32_t left = a.n_out - c0;
+            float v[16];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                i4 acc = {0, 0, 0, 0};
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(lw[((nb * 4 + t) * KC + kc) * 64 + lane], q[kc], acc, 0, 0, 0);
+                const uint32_t c = nb * 64 + channel_of(t, g, wide);
+                const vec<float, 4> ws = *(const vec<float, 4>*)(lscale + c), b = *(const vec<float, 4>*)(lbias + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 * t + i] = finish(acc[i], ws[i], scale, b[i], low);
+            }
+            if (row >= tile.end) continue;
+            if constexpr (!WHOLE) store_block(a, row, c0, g, v, left, aligned && left >= 64);
+            else if constexpr (YT == DT_F32) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t c = channel_of(t, g, true);
+                    if (c < left) *(vec<float, 4>*)((float*)a.y + (uint64_t)row * a.ld_y + c0 + c) = vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+                }
+            } else {
+                using T = std::conditional_t<YT == DT_F16, _Float16, __bf16>;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint32_t c = channel_of(2 * p, g, false);
+                    vec<T, 8> o;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = (T)v[8 * p + i];
+                    if (c < left) *(vec<T, 8>*)((T*)a.y + (uint64_t)row * a.ld_y + c0 + c) = o;
+                }
+            }
+        }
+    }
+}
+
+template <int DT, int YT, int KC>
+static void linear_rows(const LinearArgs& a, hipStream_t s) {
+    // Rows a workgroup: few where there are few, so that the chip is filled; else 128 (2^20 x 64 -> 64: 52.8 us; with 256 rows 55.7, with 512
+    // 61.8).
+    uint32_t shift = 6;
+    if ((a.rows >> shift) > 2048) ++shift;
+    const uint32_t nb = a.n_out <= 64 ? 1 : a.n_out <= 128 && YT >= 0 ? 2 : 4;
+    const dim3 grid(row_tiles(a, shift), (a.n_out + nb * 64 - 1) / (nb * 64));
+    if (nb == 1) linear_i8_rows_kernel<DT, YT, KC, 1><<<grid, 256, 0, s>>>(a, shift);
+    else if constexpr (YT >= 0) {
+        if (nb == 2) linear_i8_rows_kernel<DT, YT, KC, 2><<<grid, 256, 0, s>>>(a, shift);
+    }
+    if (nb == 4) linear_i8_rows_kernel<DT, YT, KC, 4><<<grid, 256, 0, s>>>(a, shift);
+}
+template <int DT, int YT>
+static void linear_rows_of(const LinearArgs& a, hipStream_t s) {
+    if (a.n_in <= 64) linear_rows<DT, YT, 1>(a, s);
+    else if (a.n_in <= 128) linear_rows<DT, YT, 2>(a, s);
+    else linear_rows<DT, YT, 4>(a, s);
+}
+template <int DT>
+static void linear_rows_by_type(const LinearArgs& a, hipStream_t s) {
+    const uint64_t y_bytes = a.y_dtype == DT_F32 ? 4 : 2;
+    const bool whole = a.n_in % 16 == 0 && a.n_out % 8 == 0 && ((uint64_t)a.y | a.ld_y * y_bytes) % 16 == 0;
+    if constexpr (DT == DT_I8) {
+        if (whole && a.y_dtype == DT_F16) return linear_rows_of<DT, DT_F16>(a, s);
+        if (whole && a.y_dtype == DT_BF16) return linear_rows_of<DT, DT_BF16>(a, s);
+        if (whole) return linear_rows_of<DT, DT_F32>(a, s);
+    } else if (whole && a.y_dtype == DT) return linear_rows_of<DT, DT>(a, s);   // (a layer's output is its input's type; others: the general one)
+    linear_rows_of<DT, -1>(a, s);
+}
+
+void launch_linear_rows(const LinearArgs& a, hipStream_t s) {
+    by_type(a.x_dtype, [&](auto t) { linear_rows_by_type<decltype(t)::value>(a, s); });
+}
+
+}  // namespace sng
