@@ -145,7 +145,7 @@ void quantize_rows_i8(sng_ctx* c, const void* x, int32_t dtype, uint32_t rows, u
 uint64_t linear_i8_workspace(uint32_t rows, uint32_t n_in, uint32_t n_out, int32_t x_dtype, uint32_t n_experts) {
     check_linear(rows, n_in, n_out, n_experts);
     check_type(x_dtype, true);
-    if (rows == 0 || x_dtype == SNG_I8 || linear_i8_quantizes(linear_i8_kernel(rows, n_in, n_out, n_experts), rows, n_experts)) return 0;
+    if (rows == 0 || x_dtype == SNG_I8 || linear_i8_quantizes(rows, n_in, n_out, n_experts)) return 0;
     return rows * padded(n_in) + (uint64_t)rows * sizeof(float);
 }
 

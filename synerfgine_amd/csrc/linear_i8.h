@@ -151,10 +151,10 @@ static uint32_t row_tiles(const LinearArgs& a, uint32_t shift) {
 // 16 elements of a row of n >= 16 from element k on (a multiple of 16), at any alignment and without reading behind the
 // row: the row's last 16 are read where fewer are left.  keep_inside then moves those to their places and clears what lies
 // from n on.  Two steps, so that all of a thread's loads are on their way before it waits for the first.
-template <int DT>
+template <int DT, bool INSIDE = false>   // INSIDE: k + 16 <= n
 __device__ __forceinline__ Raw<DT, 16> load_row16(const char* __restrict__ row, uint32_t k, uint32_t n) {
     Raw<DT, 16> r;
-    __builtin_memcpy(&r, row + (uint64_t)min(k, n - 16) * bytes_of(DT), sizeof(r));
+    __builtin_memcpy(&r, row + (uint64_t)(INSIDE ? k : min(k, n - 16)) * bytes_of(DT), sizeof(r));
     return r;
 }
 template <int DT, bool WHOLE = false>   // WHOLE: n is a multiple of 16
@@ -247,6 +247,7 @@ __device__ __forceinline__ bool y_aligned(const LinearArgs& a) { return (((uint6
 
 void launch_linear_rows(const LinearArgs& a, hipStream_t s);   // n_in <= 256
 void launch_linear_few(const LinearArgs& a, hipStream_t s);
+bool linear_few_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_experts);
 
 // f(the x type as a constant)
 template <typename F>

@@ -318,7 +318,10 @@ LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint
     if (rows <= 16u * n_experts) return LinearKernel::Few;
     return LinearKernel::Tile;
 }
-bool linear_i8_quantizes(LinearKernel k, uint32_t rows, uint32_t n_experts) { return k != LinearKernel::Tile; }
+bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
+    const LinearKernel k = linear_i8_kernel(rows, n_in, n_out, n_experts);
+    return k == LinearKernel::Rows || (k == LinearKernel::Few && linear_few_quantizes(rows, n_in, n_experts));
+}
 
 void launch_linear_i8(const LinearArgs& a, hipStream_t s) {
     switch (linear_i8_kernel(a.rows, a.n_in, a.n_out, a.n_experts)) {
@@ -331,7 +334,8 @@ void launch_linear_i8(const LinearArgs& a, hipStream_t s) {
         const uint64_t cells = (uint64_t)a.rows * a.n_out;
         if (cells >= 192ull * 256 * 256) linear_stream<256, 256, 2, 2>(a, s);
         else if (cells >= 192ull * 128 * 128) linear_stream<128, 128, 2, 2>(a, s);
-        else linear_stream<64, 128, 2, 4>(a, s);
+        else if (cells >= 96ull * 64 * 128) linear_stream<64, 128, 2, 4>(a, s);
+        else linear_stream<64, 64, 4, 4>(a, s);
         return;
     }
     if (a.y_dtype == DT_F16) linear<_Float16>(a, s);

@@ -5,13 +5,22 @@ namespace sng {
 
 // Bound by reading the weights once, and for the smallest by the chain of waits.  A workgroup takes 16 CT channels of one
 // matrix and splits n_in over its NW waves, so that a whole chip of waves is loading also for one row; each wave's sums meet
-// in LDS.  x (up to 16 rows at a time) is brought to 8 bits on the way: every wave reads its own part of the rows, the
-// waves share the rows' maxima in LDS.  Everything that a wave of up to H fragments needs is on its way before it waits for
-// the first time: weights, rows, scales.
-template <int DT, int NW, int H, int CT>   // H fragments of 64 bytes at a time
-__global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a) {
-    constexpr int XB = bytes_of(DT), RESULTS = CT * 256 / (NW * 64) > 0 ? CT * 256 / (NW * 64) : 1;
-    __shared__ uint32_t tops[NW][16];
+// in LDS.  x (up to 16 rows at a time) in floating point is brought to 8 bits on the way, by all waves together, into LDS,
+// where the fragments are read from: with few rows most lanes of a fragment would have none to work on.  Every workgroup does
+// that again, which is little beside its weights.  The rows are asked for first and the first weights right behind them:
+// loads come back in their order, and the weights have the time that the rows' way to 8 bits takes.
+//
+// A call runs every instruction about once, out of a cold instruction cache: what is repeated is a loop, and sizes that
+// need no clearing behind the rows' ends (WHOLE: n_in in 64s) have a kernel without the code for it.  (1 x 4096 -> 4096:
+// 12.1 us with that code between the matrix instructions, each jump over it a miss.)
+constexpr uint32_t FEW_LDS = 60 * 1024;   // for x's rows
+static uint32_t few_stride(uint32_t n_in) { return (n_in + 63) / 64 * 64 + 16; }   // (+ 16: the rows of a fragment read lie on different banks)
+
+template <int DT, int NW, int H, int CT, bool WHOLE>   // H fragments of 64 bytes at a time
+__global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, uint32_t group, uint32_t stride) {
+    constexpr int XB = bytes_of(DT), T = NW * 64, RESULTS = CT * 256 / T > 0 ? CT * 256 / T : 1;
+    extern __shared__ __align__(16) int8_t lq[];   // [group][stride]
+    __shared__ uint32_t tops[16][NW];
     __shared__ i4 sums[NW][CT][64];
     const uint32_t expert = blockIdx.y;
     uint32_t begin = 0, end = a.rows;
@@ -20,81 +29,90 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a) {
         end = min((uint32_t)a.offsets[expert + 1], a.rows);
         if (begin >= end) return;
     }
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-    const uint32_t n0 = blockIdx.x * (16 * CT), steps = (a.n_in + 63) / 64, per = (steps + NW - 1) / NW;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15, n = a.n_in;
+    const uint32_t n0 = blockIdx.x * (16 * CT), steps = (n + 63) / 64, per = (steps + NW - 1) / NW;
     const uint32_t s0 = min(steps, wave * per), s1 = min(steps, s0 + per);
-    const int8_t* w[CT];
+    const char* w[CT];
 #pragma unroll
-    for (int t = 0; t < CT; ++t) w[t] = a.w + ((uint64_t)expert * a.n_out + min(n0 + t * 16 + r, a.n_out - 1)) * a.ld_w;
-    // steps past this wave's last are read as its last and not multiplied; fragments are cleared past the row's end
+    for (int t = 0; t < CT; ++t) w[t] = (const char*)a.w + ((uint64_t)expert * a.n_out + min(n0 + t * 16 + r, a.n_out - 1)) * a.ld_w;
+    // steps past this wave's last are read as its last and not multiplied
     const auto load_w = [&](uint32_t s, Raw<DT_I8, 16> (&f)[H][CT]) {
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int t = 0; t < CT; ++t) f[h][t] = load_row16<DT_I8>((const char*)w[t], min(s + h, s1 - 1) * 64 + g * 16, a.n_in);
+            for (int t = 0; t < CT; ++t) f[h][t] = load_row16<DT_I8, WHOLE>(w[t], min(s + h, s1 - 1) * 64 + g * 16, n);
     };
-    const bool ragged = a.n_in % 64 != 0;
-    // this thread's results: row (i / 16) % 16, channel i / 256 * 16 + i % 16 for i = tid + k NW 64
+    // x's units of 16 values: a row's lie on WPR waves (several a thread where it has more), RPP rows a pass
+    const uint32_t units = steps * 4, wpr = min((units + 63) / 64, (uint32_t)NW), rpp = NW / wpr, my_row = wave / wpr, my_unit = (wave % wpr) * 64 + lane;
+    // this thread's results: row (i / 16) % 16, channel i / 256 * 16 + i % 16 for i = tid + k T
     float w_scale[RESULTS], bias[RESULTS];
-    const auto channel = [&](int k) { return n0 + (threadIdx.x + k * NW * 64) / 256 * 16 + (threadIdx.x & 15); };
+    const auto channel = [&](int k) { return n0 + (threadIdx.x + k * T) / 256 * 16 + (threadIdx.x & 15); };
 #pragma unroll
     for (int k = 0; k < RESULTS; ++k) {
         const uint64_t at = (uint64_t)expert * a.n_out + min(channel(k), a.n_out - 1);
         w_scale[k] = a.w_scale[at];
         bias[k] = a.bias ? a.bias[at] : 0.0f;
     }
-    const float low = lowest(a);
-    for (uint32_t row0 = begin; row0 < end; row0 += 16) {
-        const uint32_t row = row0 + r;
-        const bool on = row < end;
-        const char* __restrict__ x = (const char*)a.x + (uint64_t)(on ? row : row0) * a.ld_x * XB;
-        const auto load_x = [&](uint32_t s, Raw<DT, 16> (&f)[H]) {
-#pragma unroll
-            for (int h = 0; h < H; ++h) f[h] = load_row16<DT>(x, min(s + h, s1 - 1) * 64 + g * 16, a.n_in);
-        };
+    for (uint32_t row0 = begin; row0 < end; row0 += group) {
+        const uint32_t rows = min(group, end - row0);
         Raw<DT_I8, 16> fw[H][CT];
-        Raw<DT, 16> fx[H];
-        i4 acc[CT] = {};
-        if (s0 < s1) {   // (a wave without a part only meets the others)
-            if (on) load_x(s0, fx);
-            load_w(s0, fw);
-        }
-        RowScale rs = {};
-        if constexpr (DT != DT_I8) {
-            uint32_t top = 0;
-            if (on && s0 < s1) {   // (elements read for others' places are the row's own too)
+        if constexpr (DT == DT_I8) {
+            if (s0 < s1) load_w(s0, fw);   // (a wave without a part only meets the others)
+        } else {
+            const auto get = [&](uint32_t row, uint32_t u) { return load_row16<DT, WHOLE>((const char*)a.x + (uint64_t)(row0 + row) * a.ld_x * XB, u * 16, n); };
+            const bool one = rows <= rpp && units <= wpr * 64;   // one unit a thread: it stays in registers
+            Raw<DT, 16> held = {};
+            if (my_row < rows && my_unit < units) held = get(my_row, my_unit);
+            if (s0 < s1) load_w(s0, fw);
+            // (a wave without a row of its own in a pass: none)
+#pragma unroll 1
+            for (uint32_t row = my_row < rpp ? my_row : rows; row < rows; row += rpp) {
+                uint32_t top = 0;
+#pragma unroll 1
+                for (uint32_t u = my_unit; u < units; u += wpr * 64) {
+                    if (!one) held = get(row, u);
+                    top = max(top, top_bits(held));
+                }
 #pragma unroll
-                for (int h = 0; h < H; ++h) top = max(top, top_bits(fx[h]));
-                for (uint32_t s = s0 + H; s < s1; ++s) top = max(top, top_bits(load_row16<DT>(x, s * 64 + g * 16, a.n_in)));
+                for (int m = 32; m > 0; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
+                if (lane == 0) tops[row][wave % wpr] = top;
             }
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-            if (g == 0) tops[wave][r] = top;
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < NW; ++i) top = max(top, tops[i][r]);
-            rs = row_scale(top);
-        }
-        for (uint32_t s = s0; s < s1; s += H) {
-            if (s > s0) {
-                if (on) load_x(s, fx);
-                load_w(s, fw);
+#pragma unroll 1
+            for (uint32_t row = my_row < rpp ? my_row : rows; row < rows; row += rpp) {
+                uint32_t top = 0;
+#pragma unroll 1
+                for (uint32_t i = 0; i < wpr; ++i) top = max(top, tops[row][i]);
+                const RowScale rs = row_scale(top);
+#pragma unroll 1
+                for (uint32_t u = my_unit; u < units; u += wpr * 64) {
+                    if (!one) held = get(row, u);
+                    if (!WHOLE) keep_inside<DT>(held, u * 16, n);
+                    *(i4*)(lq + row * stride + u * 16) = quantize_n(held, rs);
+                }
             }
+            __syncthreads();
+        }
+        i4 acc[CT] = {};
+        for (uint32_t s = s0; s < s1; s += H) {
+            Raw<DT_I8, 16> fx[H];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const uint32_t k = min(s + h, s1 - 1) * 64 + g * 16;
-                i4 q = {0, 0, 0, 0};
-                if (on) {   // (most lanes have no row when there are few)
-                    if (ragged) keep_inside<DT>(fx[h], k, a.n_in);
-                    if constexpr (DT == DT_I8) q = as_fragment(fx[h]);
-                    else q = quantize_n(fx[h], rs);
-                }
-                if (s + h < s1)
+                const uint32_t k = min(s + h, s1 - 1) * 64 + g * 16, row = min(r, rows - 1);
+                if constexpr (DT == DT_I8) fx[h] = load_row16<DT_I8, WHOLE>((const char*)a.x + (uint64_t)(row0 + row) * a.ld_x, k, n);
+                else __builtin_memcpy(&fx[h], __builtin_assume_aligned(lq + row * stride + k, 16), 16);
+            }
+            if (s > s0) load_w(s, fw);
 #pragma unroll
-                    for (int t = 0; t < CT; ++t) {
-                        if (ragged) keep_inside<DT_I8>(fw[h][t], k, a.n_in);
-                        acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as_fragment(fw[h][t]), q, acc[t], 0, 0, 0);
-                    }
+            for (int h = 0; h < H; ++h) {
+                if (s + h >= s1) break;
+                const uint32_t k = (s + h) * 64 + g * 16;
+                if (DT == DT_I8 && !WHOLE) keep_inside<DT_I8>(fx[h], k, n);   // (x's zeros are enough, but the weights' last pieces have to be moved)
+#pragma unroll
+                for (int t = 0; t < CT; ++t) {
+                    if (!WHOLE) keep_inside<DT_I8>(fw[h][t], k, n);
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as_fragment(fw[h][t]), as_fragment(fx[h]), acc[t], 0, 0, 0);
+                }
             }
         }
 #pragma unroll
@@ -102,41 +120,50 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a) {
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < RESULTS; ++k) {
-            const uint32_t i = threadIdx.x + k * NW * 64, rr = (i >> 4) & 15, c = i & 15;
-            if (i < CT * 256 && row0 + rr < end && channel(k) < a.n_out) {   // lane 16 (c / 4) + row held sum c % 4
+            const uint32_t i = threadIdx.x + k * T, rr = (i >> 4) & 15, c = i & 15;
+            if (i < CT * 256 && rr < rows && channel(k) < a.n_out) {   // lane 16 (c / 4) + row held sum c % 4
                 int sum = 0;
-                uint32_t top = 0;
 #pragma unroll
-                for (int j = 0; j < NW; ++j) {
-                    sum += ((const int*)&sums[j][i >> 8][(c >> 2) * 16 + rr])[c & 3];
-                    if constexpr (DT != DT_I8) top = max(top, tops[j][rr]);
+                for (int j = 0; j < NW; ++j) sum += ((const int*)&sums[j][i >> 8][(c >> 2) * 16 + rr])[c & 3];
+                float scale;
+                if constexpr (DT == DT_I8) scale = a.x_scale[row0 + rr];
+                else {
+                    uint32_t top = 0;
+#pragma unroll 1
+                    for (uint32_t j = 0; j < wpr; ++j) top = max(top, tops[rr][j]);
+                    scale = scale_of(top);
                 }
-                const float v = finish(sum, w_scale[k], DT == DT_I8 ? a.x_scale[row0 + rr] : scale_of(top), bias[k], low);
+                const float v = finish(sum, w_scale[k], scale, bias[k], lowest(a));
                 const uint64_t to = (uint64_t)(row0 + rr) * a.ld_y + channel(k);
                 if (a.y_dtype == DT_F16) ((_Float16*)a.y)[to] = (_Float16)v;
                 else if (a.y_dtype == DT_BF16) ((__bf16*)a.y)[to] = (__bf16)v;
                 else ((float*)a.y)[to] = v;
             }
         }
-        __syncthreads();
+        if (row0 + group < end) __syncthreads();
     }
+}
+
+template <int DT, int CT, bool WHOLE>
+static void linear_few_of(const LinearArgs& a, hipStream_t s) {
+    const uint32_t stride = few_stride(a.n_in), group = DT == DT_I8 ? 16 : std::min(16u, FEW_LDS / stride), lds = DT == DT_I8 ? 0 : group * stride;
+    const dim3 grid((a.n_out + 16 * CT - 1) / (16 * CT), a.offsets ? a.n_experts : 1);
+    if (a.n_in <= 1024) linear_i8_few_kernel<DT, 4, 4, CT, WHOLE><<<grid, 256, lds, s>>>(a, group, stride);
+    else linear_i8_few_kernel<DT, 8, (CT > 1 ? 4 : 8), CT, WHOLE><<<grid, 512, lds, s>>>(a, group, stride);
 }
 
 template <int DT>
 static void linear_few(const LinearArgs& a, hipStream_t s) {
-    const uint32_t experts = a.offsets ? a.n_experts : 1;
-    constexpr int H8 = DT == DT_F32 ? 4 : 8;   // (registers)
-    if ((uint64_t)a.n_out * experts > 1024 * 16) {   // more workgroups than the chip holds at once: twice the channels each
-        const dim3 grid((a.n_out + 31) / 32, experts);
-        if (a.n_in <= 1024) linear_i8_few_kernel<DT, 4, 4, 2><<<grid, 256, 0, s>>>(a);
-        else linear_i8_few_kernel<DT, 8, 4, 2><<<grid, 512, 0, s>>>(a);
-    } else {
-        const dim3 grid((a.n_out + 15) / 16, experts);
-        if (a.n_in <= 1024) linear_i8_few_kernel<DT, 4, 4, 1><<<grid, 256, 0, s>>>(a);
-        else linear_i8_few_kernel<DT, 8, H8, 1><<<grid, 512, 0, s>>>(a);
-    }
+    // more workgroups than the chip holds at once: twice the channels each
+    const bool many = (uint64_t)a.n_out * (a.offsets ? a.n_experts : 1) > 1024 * 16;
+    if (a.n_in % 64 == 0) many ? linear_few_of<DT, 2, true>(a, s) : linear_few_of<DT, 1, true>(a, s);
+    else many ? linear_few_of<DT, 2, false>(a, s) : linear_few_of<DT, 1, false>(a, s);
 }
 
+// whether the rows of a group fit LDS: else they are brought to 8 bits before
+bool linear_few_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_experts) {
+    return std::min(16u, FEW_LDS / few_stride(n_in)) >= (n_experts == 1 ? rows : 8u);
+}
 void launch_linear_few(const LinearArgs& a, hipStream_t s) {
     by_type(a.x_dtype, [&](auto t) { linear_few<decltype(t)::value>(a, s); });
 }

@@ -92,7 +92,7 @@ struct LinearArgs {
 enum class LinearKernel { Rows, Few, Tile };
 LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts);
 // whether the kernel brings x to 8 bits itself (else x has to be DT_I8)
-bool linear_i8_quantizes(LinearKernel k, uint32_t rows, uint32_t n_experts);
+bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts);
 void launch_quantize_rows(const QuantArgs& a, hipStream_t s);
 void launch_linear_i8(const LinearArgs& a, hipStream_t s);
 
