@@ -25,21 +25,24 @@ __device__ __forceinline__ void wave_ranks(const int32_t* __restrict__ ids, uint
         const uint32_t id = i < total ? (uint32_t)ids[i] : 0xffffffffu;
         key[r] = id < n_experts ? id : 0xffffffffu;
     }
+    // the counters' answers are asked for in all rounds before the first is waited for
+    unsigned long long peers[ROUNDS];
+    uint32_t old[ROUNDS];
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
         const bool kept = key[r] != 0xffffffffu;
-        unsigned long long peers = __ballot(kept);
+        peers[r] = __ballot(kept);
         for (int b = 0; b < id_bits; ++b) {
             const bool bit = (key[r] >> b) & 1u;
             const unsigned long long m = __ballot(bit);
-            peers &= bit ? m : ~m;
+            peers[r] &= bit ? m : ~m;
         }
-        uint32_t old = 0;
-        const int leader = kept ? __ffsll(peers) - 1 : lane;
-        if (kept && leader == lane) old = atomicAdd(&cnt[key[r]], (uint32_t)__popcll(peers));
-        old = __shfl(old, leader, 64);
-        rank[r] = old + (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
+        old[r] = 0;
+        if (kept && (peers[r] & ((1ull << lane) - 1ull)) == 0) old[r] = atomicAdd(&cnt[key[r]], (uint32_t)__popcll(peers[r]));
     }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        rank[r] = __shfl(old[r], key[r] != 0xffffffffu ? __ffsll(peers[r]) - 1 : lane, 64) + (uint32_t)__popcll(peers[r] & ((1ull << lane) - 1ull));
 }
 
 // exclusive scan of one value per thread over a workgroup of NW waves; `all` receives the sum
@@ -113,72 +116,118 @@ __global__ __launch_bounds__(NW * 64) void expert_sort_one_kernel(SortArgs a, in
 }
 
 // Three launches: counts per (workgroup, expert); their exclusive sums down the workgroups; ranks and the plan.
-__global__ __launch_bounds__(256) void expert_count_kernel(SortArgs a) {
-    extern __shared__ uint32_t cnt[];
-    for (uint32_t e = threadIdx.x; e < a.n_experts; e += 256) cnt[e] = 0;
-    __syncthreads();
+__global__ __launch_bounds__(256) void expert_count_kernel(SortArgs a, int copies) {
+    extern __shared__ uint32_t cnt[];   // [copies][n_experts]: a wave's own counters where they fit, so that fewer adds meet
+    for (uint32_t e = threadIdx.x; e < copies * a.n_experts; e += 256) cnt[e] = 0;
     const uint32_t begin = blockIdx.x * SORT_CHUNK;
+    uint32_t id[SORT_CHUNK / 256];
 #pragma unroll
     for (int r = 0; r < (int)(SORT_CHUNK / 256); ++r) {
         const uint32_t i = begin + r * 256 + threadIdx.x;
-        const uint32_t id = i < a.total ? (uint32_t)a.experts[i] : 0xffffffffu;
-        if (id < a.n_experts) atomicAdd(&cnt[id], 1u);
+        id[r] = i < a.total ? (uint32_t)a.experts[i] : 0xffffffffu;
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < a.n_experts; e += 256) a.counts[(size_t)blockIdx.x * a.n_experts + e] = cnt[e];
+    uint32_t* mine = cnt + ((threadIdx.x >> 6) & (copies - 1)) * a.n_experts;
+#pragma unroll
+    for (int r = 0; r < (int)(SORT_CHUNK / 256); ++r)
+        if (id[r] < a.n_experts) atomicAdd(&mine[id[r]], 1u);
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.n_experts; e += 256) {
+        uint32_t sum = cnt[e];
+        for (int c = 1; c < copies; ++c) sum += cnt[c * a.n_experts + e];
+        a.counts[(size_t)blockIdx.x * a.n_experts + e] = sum;
+    }
 }
 
-// 64 experts per workgroup, 16 runs of workgroup counts each: a run's sum, the runs' exclusive scan in LDS, the prefixes
+// 64 experts per workgroup, 16 runs of workgroup counts each: a run's sum, the runs' exclusive scan in LDS, the prefixes.
+// Up to HELD counts of a run stay in registers, all of them asked for at once; longer runs are read twice.
 __global__ __launch_bounds__(1024) void expert_scan_kernel(SortArgs a, uint32_t blocks) {
+    constexpr uint32_t HELD = 32;
     __shared__ uint32_t sums[16][64];
-    const uint32_t e = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6;
+    const uint32_t column = threadIdx.x & 63, e = min(blockIdx.x * 64 + column, a.n_experts - 1), run = threadIdx.x >> 6;
     const uint32_t per = (blocks + 15) / 16, b0 = min(blocks, run * per), b1 = min(blocks, b0 + per);
-    const bool on = e < a.n_experts;
-    uint32_t sum = 0;
-    if (on)
+    const bool on = blockIdx.x * 64 + column < a.n_experts;
+    uint32_t* __restrict__ counts = a.counts + e;
+    uint32_t held[HELD], sum = 0;
+    if (per <= HELD) {
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i) held[i] = counts[(size_t)min(b0 + i, blocks - 1) * a.n_experts];
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i) {
+            if (b0 + i >= b1) held[i] = 0;
+            sum += held[i];
+        }
+    } else
 #pragma unroll 8
-        for (uint32_t b = b0; b < b1; ++b) sum += a.counts[(size_t)b * a.n_experts + e];
-    sums[run][threadIdx.x & 63] = sum;
+        for (uint32_t b = b0; b < b1; ++b) sum += counts[(size_t)b * a.n_experts];
+    sums[run][column] = sum;
     __syncthreads();
     uint32_t at = 0;
-    for (uint32_t r = 0; r < run; ++r) at += sums[r][threadIdx.x & 63];
+    for (uint32_t r = 0; r < run; ++r) at += sums[r][column];
     if (!on) return;
-    if (run == 15) a.counts[(size_t)blocks * a.n_experts + e] = at + sum;
+    if (run == 15) counts[(size_t)blocks * a.n_experts] = at + sum;
+    if (per <= HELD) {
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i) {
+            if (b0 + i < b1) counts[(size_t)(b0 + i) * a.n_experts] = at;
+            at += held[i];
+        }
+    } else
 #pragma unroll 8
-    for (uint32_t b = b0; b < b1; ++b) {
-        const uint32_t c = a.counts[(size_t)b * a.n_experts + e];
-        a.counts[(size_t)b * a.n_experts + e] = at;
-        at += c;
-    }
+        for (uint32_t b = b0; b < b1; ++b) {
+            const uint32_t c = counts[(size_t)b * a.n_experts];
+            counts[(size_t)b * a.n_experts] = at;
+            at += c;
+        }
 }
 
-__global__ __launch_bounds__(256) void expert_place_kernel(SortArgs a, uint32_t blocks, int id_bits) {
-    extern __shared__ uint32_t cnt[];   // [4][n_experts]
-    __shared__ uint32_t wave_sums[4];
+// The rows' order goes out through LDS: a wave's lanes hold choices of as many experts as there are, and a store of theirs
+// would touch as many lines; in the workgroup's own sorted order consecutive lanes write consecutive places.
+template <int NW>
+__global__ __launch_bounds__(NW * 64) void expert_place_kernel(SortArgs a, uint32_t blocks, int id_bits) {
+    extern __shared__ uint32_t cnt[];   // [NW][n_experts], then [n_experts]: what to add to a place in the workgroup for the place in all
+    __shared__ uint32_t wave_sums[NW];
+    __shared__ uint32_t sorted[SORT_CHUNK];   // choice in the chunk (12 bits), expert
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t e_n = a.n_experts;
-    constexpr int ROUNDS = SORT_CHUNK / 256;
-    for (uint32_t i = threadIdx.x; i < 4 * e_n; i += 256) cnt[i] = 0;
+    constexpr int ROUNDS = SORT_CHUNK / (NW * 64);
+    uint32_t* shift = cnt + NW * e_n;
+    uint32_t total = 0, before = 0;   // of this thread's expert: asked for long before they are wanted
+    const auto ask = [&](uint32_t e) {
+        total = e < e_n ? a.counts[(size_t)blocks * e_n + e] : 0u;
+        before = e < e_n ? a.counts[(size_t)blockIdx.x * e_n + e] : 0u;
+    };
+    ask(threadIdx.x);
+    for (uint32_t i = threadIdx.x; i < NW * e_n; i += NW * 64) cnt[i] = 0;
     __syncthreads();
     uint32_t key[ROUNDS], rank[ROUNDS];
-    const uint32_t begin = blockIdx.x * SORT_CHUNK + wave * (ROUNDS * 64);
+    const uint32_t chunk = blockIdx.x * SORT_CHUNK, begin = chunk + wave * (ROUNDS * 64);
     wave_ranks<ROUNDS>(a.experts, begin, a.total, e_n, id_bits, cnt + wave * e_n, lane, key, rank);
     __syncthreads();
-    uint32_t base = 0;
-    for (uint32_t e0 = 0; e0 < e_n; e0 += 256) {
+    uint32_t base = 0, local_base = 0;
+    for (uint32_t e0 = 0; e0 < e_n; e0 += NW * 64) {
         const uint32_t e = e0 + threadIdx.x;
-        uint32_t all;
-        const uint32_t first = base + block_scan<4>(e < e_n ? a.counts[(size_t)blocks * e_n + e] : 0u, wave_sums, all);
+        if (e0 > 0) ask(e);
+        uint32_t c[NW], here = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) c[w] = e < e_n ? cnt[w * e_n + e] : 0u;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) here += c[w];
+        uint32_t all, all_here;
+        const uint32_t local = local_base + block_scan<NW>(here, wave_sums, all_here);
+        const uint32_t first = base + block_scan<NW>(total, wave_sums, all);
         if (e < e_n) {
             if (blockIdx.x == 0) a.offsets[e] = (int32_t)first;
-            uint32_t at = first + a.counts[(size_t)blockIdx.x * e_n + e];
-            for (int w = 0; w < 4; ++w) {
-                const uint32_t c = cnt[w * e_n + e];
+            shift[e] = first + before - local;
+            uint32_t at = local;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
                 cnt[w * e_n + e] = at;
-                at += c;
+                at += c[w];
             }
         }
         base += all;
+        local_base += all_here;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[e_n] = (int32_t)base;
     __syncthreads();
@@ -188,11 +237,14 @@ __global__ __launch_bounds__(256) void expert_place_kernel(SortArgs a, uint32_t 
         if (i >= a.total) continue;
         const bool kept = key[r] != 0xffffffffu;
         const uint32_t at = kept ? cnt[wave * e_n + key[r]] + rank[r] : 0;
-        a.slot[i] = kept ? (int32_t)at : -1;
-        if (kept) a.order[at] = (int32_t)i;
+        a.slot[i] = kept ? (int32_t)(at + shift[key[r]]) : -1;
+        if (kept) sorted[at] = key[r] << 12 | (i - chunk);
         if (i >= base) a.order[i] = -1;
     }
+    __syncthreads();
+    for (uint32_t l = threadIdx.x; l < local_base; l += NW * 64) a.order[l + shift[sorted[l] >> 12]] = (int32_t)(chunk + (sorted[l] & 4095u));
 }
+static_assert(SORT_CHUNK == 4096 && EXPERTS_MAX <= 1 << 20, "a choice of the chunk and its expert share 32 bits");
 
 void launch_expert_sort(const SortArgs& a, hipStream_t s) {
     int id_bits = 0;
@@ -203,9 +255,13 @@ void launch_expert_sort(const SortArgs& a, hipStream_t s) {
         expert_sort_one_kernel<16, 16><<<1, 1024, 16 * a.n_experts * 4, s>>>(a, id_bits);
     else {
         const uint32_t blocks = sort_blocks(a.total);
-        expert_count_kernel<<<blocks, 256, a.n_experts * 4, s>>>(a);
+        const int copies = a.n_experts <= 1024 ? 4 : 1;
+        expert_count_kernel<<<blocks, 256, copies * a.n_experts * 4, s>>>(a, copies);
         expert_scan_kernel<<<(a.n_experts + 63) / 64, 1024, 0, s>>>(a, blocks);
-        expert_place_kernel<<<blocks, 256, 4 * a.n_experts * 4, s>>>(a, blocks, id_bits);
+        // (as many waves as have counters of their own in 64 KiB of LDS beside the 16 KiB of sorted choices)
+        if (a.n_experts <= 1024) expert_place_kernel<8><<<blocks, 512, 9 * a.n_experts * 4, s>>>(a, blocks, id_bits);
+        else if (a.n_experts <= 2048) expert_place_kernel<4><<<blocks, 256, 5 * a.n_experts * 4, s>>>(a, blocks, id_bits);
+        else expert_place_kernel<2><<<blocks, 128, 3 * a.n_experts * 4, s>>>(a, blocks, id_bits);
     }
 }
 
@@ -226,42 +282,58 @@ static int vector_bytes(int elem, uint32_t d, std::initializer_list<uint64_t> ad
     return elem;
 }
 
-// Rows of the sorted order gathered from the samples: consecutive threads take consecutive pieces of consecutive rows,
-// so the stores are whole lines also for 28-byte rows.
+// Each sample's row to all its places: x is read once and in order, and a row's pieces go out together.  (The other way
+// round, rows of the sorted order gathered, reads a cache line of x for each 28-byte row: 2^20 x 2 such rows 45 us.)
 template <typename T>
-__global__ __launch_bounds__(256) void expert_gather_kernel(const T* __restrict__ x, uint64_t ld_x, const int32_t* __restrict__ order, uint32_t total, FastDiv k,
-                                                            uint32_t rows_per_block, FastDiv pieces, T* __restrict__ out, uint64_t ld_out) {
-    for (uint32_t b = blockIdx.x; b * (uint64_t)rows_per_block < total; b += gridDim.x) {
-        const uint32_t p0 = b * rows_per_block, rows = min(rows_per_block, total - p0);
-        for (uint32_t i = threadIdx.x; i < rows * pieces.d; i += 256) {
-            const uint32_t r = pieces.div(i), c = i - r * pieces.d;
-            const uint32_t from = (uint32_t)order[p0 + r];
-            if (from < total) out[(uint64_t)(p0 + r) * ld_out + c] = x[(uint64_t)k.div(from) * ld_x + c];
+__global__ __launch_bounds__(256) void expert_scatter_kernel(const T* __restrict__ x, uint64_t ld_x, const int32_t* __restrict__ slot, uint32_t n, uint32_t k, uint32_t total,
+                                                             uint32_t samples_per_block, FastDiv pieces, T* __restrict__ out, uint64_t ld_out) {
+    constexpr int U = 4;
+    for (uint64_t t0 = blockIdx.x * (uint64_t)samples_per_block; t0 < n; t0 += gridDim.x * (uint64_t)samples_per_block) {
+        const uint32_t samples = min((uint64_t)samples_per_block, n - t0), count = samples * pieces.d;
+        for (uint32_t i0 = threadIdx.x; i0 < count; i0 += 256 * U) {
+            uint32_t t[U], c[U];
+            T v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t i = min(i0 + u * 256, count - 1);
+                t[u] = pieces.div(i);
+                c[u] = i - t[u] * pieces.d;
+                v[u] = x[(t0 + t[u]) * ld_x + c[u]];
+            }
+            for (uint32_t j = 0; j < k; ++j) {
+                uint32_t to[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) to[u] = (uint32_t)slot[(t0 + t[u]) * k + j];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (to[u] < total && i0 + u * 256 < count) out[(uint64_t)to[u] * ld_out + c[u]] = v[u];
+            }
         }
     }
 }
 
 template <typename T>
-static void gather(const RowsArgs& a, int elem, hipStream_t s) {
+static void scatter(const RowsArgs& a, int elem, hipStream_t s) {
     const uint32_t per = sizeof(T) / elem, pieces = a.d / per, total = a.n * a.k;
-    const uint32_t rows = std::max(1u, 1024u / pieces);
-    expert_gather_kernel<T><<<grid_of((total + rows - 1) / rows), 256, 0, s>>>((const T*)a.src, a.ld_src / per, a.order, total, FastDiv(a.k), rows, FastDiv(pieces), (T*)a.dst,
-                                                                     a.ld_dst / per);
+    const uint32_t samples = std::max(1u, 1024u / pieces);
+    expert_scatter_kernel<T><<<grid_of((a.n + samples - 1) / samples), 256, 0, s>>>((const T*)a.src, a.ld_src / per, a.slot, a.n, a.k, total, samples, FastDiv(pieces),
+                                                                                    (T*)a.dst, a.ld_dst / per);
 }
 
 void launch_expert_dispatch(const RowsArgs& a, hipStream_t s) {
     const int elem = a.dtype == DT_F32 ? 4 : a.dtype == DT_I8 ? 1 : 2;
     switch (vector_bytes(elem, a.d, {(uint64_t)a.src, (uint64_t)a.dst, a.ld_src * elem, a.ld_dst * elem})) {
-        case 16: gather<uint4>(a, elem, s); break;
-        case 8: gather<uint2>(a, elem, s); break;
-        case 4: gather<uint32_t>(a, elem, s); break;
-        case 2: gather<uint16_t>(a, elem, s); break;
-        default: gather<uint8_t>(a, elem, s); break;
+        case 16: scatter<uint4>(a, elem, s); break;
+        case 8: scatter<uint2>(a, elem, s); break;
+        case 4: scatter<uint32_t>(a, elem, s); break;
+        case 2: scatter<uint16_t>(a, elem, s); break;
+        default: scatter<uint8_t>(a, elem, s); break;
     }
 }
 
-// y[t] = sum_j w[t,j] rows[slot[t,j]], f32 in the order of j, rounded once.
-template <typename T, int N>
+// y[t] = sum_j w[t,j] rows[slot[t,j]], f32 in the order of j, rounded once.  The places and weights of J choices are asked
+// for together, then their J pieces, so that a thread waits twice for J choices and not twice for each.
+template <typename T, int N, int J>
 __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_t rows_per_block, FastDiv pieces) {
     using V = vec<T, N>;
     const uint32_t total = a.n * a.k;
@@ -269,29 +341,45 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
     V* __restrict__ dst = (V*)a.dst;
     const uint64_t ld_src = a.ld_src / N, ld_dst = a.ld_dst / N;
     for (uint32_t b = blockIdx.x; b * (uint64_t)rows_per_block < a.n; b += gridDim.x)
-    for (uint32_t i = threadIdx.x, t0 = b * rows_per_block, rows = min(rows_per_block, a.n - t0); i < rows * pieces.d; i += 256) {
-        const uint32_t r = pieces.div(i), c = i - r * pieces.d;
-        const uint32_t first = (t0 + r) * a.k;
-        float sum[N] = {};
-        for (uint32_t j = 0; j < a.k; ++j) {
-            const uint32_t at = (uint32_t)a.slot[first + j];
-            if (at >= total) continue;
-            const V v = src[(uint64_t)at * ld_src + c];
-            const float w = a.weights ? a.weights[first + j] : 1.0f;
+        for (uint32_t i = threadIdx.x, t0 = b * rows_per_block, rows = min(rows_per_block, a.n - t0); i < rows * pieces.d; i += 256) {
+            const uint32_t r = pieces.div(i), c = i - r * pieces.d;
+            const uint32_t first = (t0 + r) * a.k;
+            float sum[N] = {};
+            for (uint32_t j0 = 0; j0 < a.k; j0 += J) {
+                uint32_t at[J];
+                float w[J];
+                V v[J];
 #pragma unroll
-            for (int q = 0; q < N; ++q) sum[q] = fmaf(w, (float)v[q], sum[q]);
+                for (int j = 0; j < J; ++j) {
+                    const uint32_t i = first + min(j0 + j, a.k - 1);
+                    at[j] = (uint32_t)a.slot[i];
+                    w[j] = a.weights ? a.weights[i] : 1.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    if (j0 + j >= a.k) at[j] = total;
+                    v[j] = at[j] < total ? src[(uint64_t)at[j] * ld_src + c] : V(0);
+                }
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    if (at[j] < total)
+#pragma unroll
+                        for (int q = 0; q < N; ++q) sum[q] = fmaf(w[j], (float)v[j][q], sum[q]);
+            }
+            V y;
+#pragma unroll
+            for (int q = 0; q < N; ++q) y[q] = (T)sum[q];
+            dst[(uint64_t)(t0 + r) * ld_dst + c] = y;
         }
-        V y;
-#pragma unroll
-        for (int q = 0; q < N; ++q) y[q] = (T)sum[q];
-        dst[(uint64_t)(t0 + r) * ld_dst + c] = y;
-    }
 }
 
 template <typename T, int N>
 static void combine(const RowsArgs& a, hipStream_t s) {
-    const uint32_t pieces = a.d / N, rows = std::max(1u, 256u / pieces);
-    expert_combine_kernel<T, N><<<grid_of((a.n + rows - 1) / rows), 256, 0, s>>>(a, rows, FastDiv(pieces));
+    const uint32_t pieces = a.d / N, rows = std::max(1u, 256u / pieces), grid = grid_of((a.n + rows - 1) / rows);
+    if (a.k == 1) expert_combine_kernel<T, N, 1><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
+    else if (a.k == 2) expert_combine_kernel<T, N, 2><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
+    else if (a.k <= 4) expert_combine_kernel<T, N, 4><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
+    else expert_combine_kernel<T, N, 8><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
 }
 
 template <typename T>
