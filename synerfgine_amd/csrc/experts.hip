@@ -272,57 +272,71 @@ using vec = T __attribute__((ext_vector_type(N)));
 // HIP counts a grid's threads in 32 bits: larger grids loop
 static uint32_t grid_of(uint64_t blocks) { return (uint32_t)std::min<uint64_t>(blocks, 1u << 22); }
 
-// a thread's elements per memory access: the widest of 16, 8, 4 bytes or one element that the row length, both
-// strides and the addresses allow
-static int vector_bytes(int elem, uint32_t d, std::initializer_list<uint64_t> addresses_and_strides) {
-    uint64_t all = (uint64_t)d * elem;
-    for (uint64_t v : addresses_and_strides) all |= v;
+// A row of d elements in pieces of N, each one memory access of up to 16 bytes: the last piece ends with the row and may
+// repeat elements of the one before it (the same values, written twice).  Pieces lie at any multiple of an element, which
+// the card's loads and stores take; d = 45 in f16 goes in 6 pieces and not in 45.
+struct Pieces {
+    FastDiv count;
+    uint32_t d, n;
+    Pieces(uint32_t d, uint32_t n) : count((d + n - 1) / n), d(d), n(n) {}
+    __device__ __forceinline__ uint32_t start(uint32_t c) const { return min(c * n, d - n); }
+};
+static int piece_bytes(int elem, uint32_t d) {
     for (int b : {16, 8, 4, 2})
-        if (b > elem && all % b == 0) return b;
+        if (b > elem && (uint64_t)d * elem >= (uint64_t)b) return b;
     return elem;
 }
+template <typename V>
+__device__ __forceinline__ V get_piece(const void* p) {
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ void put_piece(void* p, const V& v) { __builtin_memcpy(p, &v, sizeof(V)); }
 
 // Each sample's row to all its places: x is read once and in order, and a row's pieces go out together.  (The other way
 // round, rows of the sorted order gathered, reads a cache line of x for each 28-byte row: 2^20 x 2 such rows 45 us.)
-template <typename T>
-__global__ __launch_bounds__(256) void expert_scatter_kernel(const T* __restrict__ x, uint64_t ld_x, const int32_t* __restrict__ slot, uint32_t n, uint32_t k, uint32_t total,
-                                                             uint32_t samples_per_block, FastDiv pieces, T* __restrict__ out, uint64_t ld_out) {
+template <typename T>   // a piece's bytes
+__global__ __launch_bounds__(256) void expert_scatter_kernel(RowsArgs a, uint32_t elem, uint32_t samples_per_block, Pieces pieces) {
     constexpr int U = 4;
-    for (uint64_t t0 = blockIdx.x * (uint64_t)samples_per_block; t0 < n; t0 += gridDim.x * (uint64_t)samples_per_block) {
-        const uint32_t samples = min((uint64_t)samples_per_block, n - t0), count = samples * pieces.d;
+    const uint32_t total = a.n * a.k;
+    const char* __restrict__ x = (const char*)a.src;
+    char* __restrict__ out = (char*)a.dst;
+    for (uint64_t t0 = blockIdx.x * (uint64_t)samples_per_block; t0 < a.n; t0 += gridDim.x * (uint64_t)samples_per_block) {
+        const uint32_t samples = min((uint64_t)samples_per_block, a.n - t0), count = samples * pieces.count.d;
         for (uint32_t i0 = threadIdx.x; i0 < count; i0 += 256 * U) {
             uint32_t t[U], c[U];
             T v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t i = min(i0 + u * 256, count - 1);
-                t[u] = pieces.div(i);
-                c[u] = i - t[u] * pieces.d;
-                v[u] = x[(t0 + t[u]) * ld_x + c[u]];
+                t[u] = pieces.count.div(i);
+                c[u] = pieces.start(i - t[u] * pieces.count.d);
+                v[u] = get_piece<T>(x + ((t0 + t[u]) * a.ld_src + c[u]) * elem);
             }
-            for (uint32_t j = 0; j < k; ++j) {
+            for (uint32_t j = 0; j < a.k; ++j) {
                 uint32_t to[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) to[u] = (uint32_t)slot[(t0 + t[u]) * k + j];
+                for (int u = 0; u < U; ++u) to[u] = (uint32_t)a.slot[(t0 + t[u]) * a.k + j];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (to[u] < total && i0 + u * 256 < count) out[(uint64_t)to[u] * ld_out + c[u]] = v[u];
+                    if (to[u] < total && i0 + u * 256 < count) put_piece(out + ((uint64_t)to[u] * a.ld_dst + c[u]) * elem, v[u]);
             }
         }
     }
 }
 
 template <typename T>
-static void scatter(const RowsArgs& a, int elem, hipStream_t s) {
-    const uint32_t per = sizeof(T) / elem, pieces = a.d / per, total = a.n * a.k;
-    const uint32_t samples = std::max(1u, 1024u / pieces);
-    expert_scatter_kernel<T><<<grid_of((a.n + samples - 1) / samples), 256, 0, s>>>((const T*)a.src, a.ld_src / per, a.slot, a.n, a.k, total, samples, FastDiv(pieces),
-                                                                                    (T*)a.dst, a.ld_dst / per);
+static void scatter(const RowsArgs& a, uint32_t elem, hipStream_t s) {
+    const Pieces pieces(a.d, sizeof(T) / elem);
+    const uint32_t samples = std::max(1u, 1024u / pieces.count.d);
+    expert_scatter_kernel<T><<<grid_of((a.n + samples - 1) / samples), 256, 0, s>>>(a, elem, samples, pieces);
 }
 
 void launch_expert_dispatch(const RowsArgs& a, hipStream_t s) {
     const int elem = a.dtype == DT_F32 ? 4 : a.dtype == DT_I8 ? 1 : 2;
-    switch (vector_bytes(elem, a.d, {(uint64_t)a.src, (uint64_t)a.dst, a.ld_src * elem, a.ld_dst * elem})) {
+    switch (piece_bytes(elem, a.d)) {
         case 16: scatter<uint4>(a, elem, s); break;
         case 8: scatter<uint2>(a, elem, s); break;
         case 4: scatter<uint32_t>(a, elem, s); break;
@@ -334,15 +348,14 @@ void launch_expert_dispatch(const RowsArgs& a, hipStream_t s) {
 // y[t] = sum_j w[t,j] rows[slot[t,j]], f32 in the order of j, rounded once.  The places and weights of J choices are asked
 // for together, then their J pieces, so that a thread waits twice for J choices and not twice for each.
 template <typename T, int N, int J>
-__global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_t rows_per_block, FastDiv pieces) {
+__global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_t rows_per_block, Pieces pieces) {
     using V = vec<T, N>;
     const uint32_t total = a.n * a.k;
-    const V* __restrict__ src = (const V*)a.src;
-    V* __restrict__ dst = (V*)a.dst;
-    const uint64_t ld_src = a.ld_src / N, ld_dst = a.ld_dst / N;
+    const T* __restrict__ src = (const T*)a.src;
+    T* __restrict__ dst = (T*)a.dst;
     for (uint32_t b = blockIdx.x; b * (uint64_t)rows_per_block < a.n; b += gridDim.x)
-        for (uint32_t i = threadIdx.x, t0 = b * rows_per_block, rows = min(rows_per_block, a.n - t0); i < rows * pieces.d; i += 256) {
-            const uint32_t r = pieces.div(i), c = i - r * pieces.d;
+        for (uint32_t i = threadIdx.x, t0 = b * rows_per_block, rows = min(rows_per_block, a.n - t0); i < rows * pieces.count.d; i += 256) {
+            const uint32_t r = pieces.count.div(i), c = pieces.start(i - r * pieces.count.d);
             const uint32_t first = (t0 + r) * a.k;
             float sum[N] = {};
             for (uint32_t j0 = 0; j0 < a.k; j0 += J) {
@@ -358,7 +371,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     if (j0 + j >= a.k) at[j] = total;
-                    v[j] = at[j] < total ? src[(uint64_t)at[j] * ld_src + c] : V(0);
+                    v[j] = at[j] < total ? get_piece<V>(src + (uint64_t)at[j] * a.ld_src + c) : V(0);
                 }
 #pragma unroll
                 for (int j = 0; j < J; ++j)
@@ -369,26 +382,26 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
             V y;
 #pragma unroll
             for (int q = 0; q < N; ++q) y[q] = (T)sum[q];
-            dst[(uint64_t)(t0 + r) * ld_dst + c] = y;
+            put_piece(dst + (uint64_t)(t0 + r) * a.ld_dst + c, y);
         }
 }
 
 template <typename T, int N>
 static void combine(const RowsArgs& a, hipStream_t s) {
-    const uint32_t pieces = a.d / N, rows = std::max(1u, 256u / pieces), grid = grid_of((a.n + rows - 1) / rows);
-    if (a.k == 1) expert_combine_kernel<T, N, 1><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
-    else if (a.k == 2) expert_combine_kernel<T, N, 2><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
-    else if (a.k <= 4) expert_combine_kernel<T, N, 4><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
-    else expert_combine_kernel<T, N, 8><<<grid, 256, 0, s>>>(a, rows, FastDiv(pieces));
+    const Pieces pieces(a.d, N);
+    const uint32_t rows = std::max(1u, 256u / pieces.count.d), grid = grid_of((a.n + rows - 1) / rows);
+    if (a.k == 1) expert_combine_kernel<T, N, 1><<<grid, 256, 0, s>>>(a, rows, pieces);
+    else if (a.k == 2) expert_combine_kernel<T, N, 2><<<grid, 256, 0, s>>>(a, rows, pieces);
+    else if (a.k <= 4) expert_combine_kernel<T, N, 4><<<grid, 256, 0, s>>>(a, rows, pieces);
+    else expert_combine_kernel<T, N, 8><<<grid, 256, 0, s>>>(a, rows, pieces);
 }
 
 template <typename T>
 static void combine_by_width(const RowsArgs& a, hipStream_t s) {
-    const int elem = sizeof(T);
-    const int b = vector_bytes(elem, a.d, {(uint64_t)a.src, (uint64_t)a.dst, a.ld_src * elem, a.ld_dst * elem});
-    if (b == 16) combine<T, 16 / sizeof(T)>(a, s);
-    else if (b == 8) combine<T, 8 / sizeof(T)>(a, s);
-    else if (b == 4) combine<T, 4 / sizeof(T)>(a, s);
+    const int n = piece_bytes(sizeof(T), a.d) / sizeof(T);
+    if (n == 8) combine<T, 8>(a, s);
+    else if (n == 4) combine<T, 4>(a, s);
+    else if (n == 2) combine<T, 2>(a, s);
     else combine<T, 1>(a, s);
 }
 
@@ -406,12 +419,11 @@ __global__ __launch_bounds__(256) void expert_combine_backward_kernel(RowsArgs a
     using V = vec<T, N>;
     constexpr int J = 4;   // choices per pass over dy
     __shared__ float part[4][J];
-    const uint32_t total = a.n * a.k, pieces = a.d / N;
+    const uint32_t total = a.n * a.k, pieces = (a.d + N - 1) / N;
     const uint32_t g = threadIdx.x % G;
-    const V* __restrict__ src = (const V*)a.src;
-    const V* __restrict__ dy = (const V*)a.dy;
-    V* __restrict__ dst = (V*)a.dst;
-    const uint64_t ld_src = a.ld_src / N, ld_dst = a.ld_dst / N, ld_dy = a.ld_dy / N;
+    const T* __restrict__ src = (const T*)a.src;
+    const T* __restrict__ dy = (const T*)a.dy;
+    T* __restrict__ dst = (T*)a.dst;
     // a group's lanes leave the loop together; with G = 256 the whole workgroup does
     for (uint64_t t = blockIdx.x * (uint64_t)(256 / G) + threadIdx.x / G; t < a.n; t += gridDim.x * (uint64_t)(256 / G))
     for (uint32_t j0 = 0; j0 < a.k; j0 += J) {
@@ -425,20 +437,21 @@ __global__ __launch_bounds__(256) void expert_combine_backward_kernel(RowsArgs a
             dot[j] = 0.0f;
         }
         for (uint32_t c = g; c < pieces; c += G) {
-            const V gv = dy[t * ld_dy + c];
+            const uint32_t at_c = min(c * N, a.d - N), seen = c * N - at_c;   // (the last piece's elements that the one before has: not summed again)
+            const V gv = get_piece<V>(dy + t * a.ld_dy + at_c);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 if (at[j] >= total) continue;
                 if (a.dweights) {
-                    const V v = src[(uint64_t)at[j] * ld_src + c];
+                    const V v = get_piece<V>(src + (uint64_t)at[j] * a.ld_src + at_c);
 #pragma unroll
-                    for (int q = 0; q < N; ++q) dot[j] = fmaf((float)gv[q], (float)v[q], dot[j]);
+                    for (int q = 0; q < N; ++q) dot[j] = (uint32_t)q >= seen ? fmaf((float)gv[q], (float)v[q], dot[j]) : dot[j];
                 }
                 if (dst) {
                     V o;
 #pragma unroll
                     for (int q = 0; q < N; ++q) o[q] = (T)(w[j] * (float)gv[q]);
-                    dst[(uint64_t)at[j] * ld_dst + c] = o;
+                    put_piece(dst + (uint64_t)at[j] * a.ld_dst + at_c, o);
                 }
             }
         }
@@ -465,7 +478,7 @@ __global__ __launch_bounds__(256) void expert_combine_backward_kernel(RowsArgs a
 
 template <typename T, int N>
 static void combine_backward(const RowsArgs& a, hipStream_t s) {
-    const uint32_t pieces = a.d / N;
+    const uint32_t pieces = (a.d + N - 1) / N;
     const auto blocks = [&](uint32_t g) { return grid_of(((uint64_t)a.n * g + 255) / 256); };
     if (pieces <= 1) expert_combine_backward_kernel<T, N, 1><<<blocks(1), 256, 0, s>>>(a);
     else if (pieces <= 4) expert_combine_backward_kernel<T, N, 4><<<blocks(4), 256, 0, s>>>(a);
@@ -476,10 +489,10 @@ static void combine_backward(const RowsArgs& a, hipStream_t s) {
 
 template <typename T>
 static void combine_backward_by_width(const RowsArgs& a, hipStream_t s) {
-    const int elem = sizeof(T);
-    const int b = vector_bytes(elem, a.d, {(uint64_t)a.src, (uint64_t)a.dst, (uint64_t)a.dy, a.ld_src * elem, a.ld_dst * elem, a.ld_dy * elem});
-    if (b == 16) combine_backward<T, 16 / sizeof(T)>(a, s);
-    else if (b >= 4) combine_backward<T, 4 / sizeof(T)>(a, s);
+    const int n = piece_bytes(sizeof(T), a.d) / sizeof(T);
+    if (n == 8) combine_backward<T, 8>(a, s);
+    else if (n == 4) combine_backward<T, 4>(a, s);
+    else if (n == 2) combine_backward<T, 2>(a, s);
     else combine_backward<T, 1>(a, s);
 }
 

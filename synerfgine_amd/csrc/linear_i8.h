@@ -197,31 +197,31 @@ __device__ __forceinline__ i4 as_fragment(const Raw<DT_I8, 16>& r) { return i4{(
 // three lanes of its row, so a store writes 64 consecutive bytes a row: 8 channels of f16 (two accumulators), 4 of f32.
 __device__ __forceinline__ uint32_t channel_of(int t, uint32_t g, bool wide) { return wide ? t * 16 + g * 4 : (t >> 1) * 32 + g * 8 + (t & 1) * 4; }
 
+// 16 bytes of y, at any place of y's type
+template <typename V>
+__device__ __forceinline__ void put_piece(void* p, const V& v) { __builtin_memcpy(p, &v, sizeof(V)); }
+template <typename T>
+__device__ __forceinline__ vec<T, 8> to_half(const float* v) {
+    vec<T, 8> o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (T)v[i];
+    return o;
+}
 // One row's 16 channels of a 64-channel block from channel c0 on (v[4 t + i], channels as channel_of says), `left` channels
-// inside; whole: all 64 are, and y takes 16-byte stores
+// inside; whole: all 64 are
 __device__ __forceinline__ void store_block(const LinearArgs& a, uint32_t row, uint32_t c0, uint32_t g, const float (&v)[16], uint32_t left, bool whole) {
     const uint64_t at = (uint64_t)row * a.ld_y + c0;
     if (whole) {
         if (a.y_dtype == DT_F32) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                *(vec<float, 4>*)((float*)a.y + at + channel_of(t, g, true)) = vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+                put_piece((float*)a.y + at + channel_of(t, g, true), vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]});
         } else if (a.y_dtype == DT_F16) {
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                vec<_Float16, 8> o;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = (_Float16)v[8 * p + i];
-                *(vec<_Float16, 8>*)((_Float16*)a.y + at + channel_of(2 * p, g, false)) = o;
-            }
+            for (int p = 0; p < 2; ++p) put_piece((_Float16*)a.y + at + channel_of(2 * p, g, false), to_half<_Float16>(v + 8 * p));
         } else {
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                vec<__bf16, 8> o;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = (__bf16)v[8 * p + i];
-                *(vec<__bf16, 8>*)((__bf16*)a.y + at + channel_of(2 * p, g, false)) = o;
-            }
+            for (int p = 0; p < 2; ++p) put_piece((__bf16*)a.y + at + channel_of(2 * p, g, false), to_half<__bf16>(v + 8 * p));
         }
         return;
     }
@@ -243,7 +243,6 @@ __device__ __forceinline__ float finish(int sum, float w_scale, float x_scale, f
     return __builtin_elementwise_maximum(fmaf((float)sum * w_scale, x_scale, bias), low);
 }
 __device__ __forceinline__ float lowest(const LinearArgs& a) { return a.relu ? 0.0f : -__builtin_inff(); }
-__device__ __forceinline__ bool y_aligned(const LinearArgs& a) { return (((uint64_t)a.y | (a.ld_y * (a.y_dtype == DT_F32 ? 4 : 2))) & 15) == 0; }
 
 void launch_linear_rows(const LinearArgs& a, hipStream_t s);   // n_in <= 256
 void launch_linear_few(const LinearArgs& a, hipStream_t s);

@@ -278,7 +278,6 @@ __global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a,
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load may reach LDS after the workgroup has left it
     const uint32_t c0 = n0 + wn;
     if (c0 >= a.n_out) return;
-    const bool aligned = y_aligned(a);
     float ws[16], b[16];
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
@@ -297,7 +296,7 @@ __global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a,
         for (int q = 0; q < 16; ++q) {
             v[q] = finish(acc[q >> 2][u][q & 3], ws[q], s, b[q], lowest(a));
         }
-        store_block(a, row, c0, g, v, a.n_out - c0, aligned && c0 + 64 <= a.n_out);
+        store_block(a, row, c0, g, v, a.n_out - c0, c0 + 64 <= a.n_out);
     }
 }
 

@@ -11,7 +11,7 @@ namespace sng {
 // loads come back in their order, and the weights have the time that the rows' way to 8 bits takes.
 //
 // A call runs every instruction about once, out of a cold instruction cache: what is repeated is a loop, and sizes that
-// need no clearing behind the rows' ends (WHOLE: n_in in 64s) have a kernel without the code for it.  (1 x 4096 -> 4096:
+// need no moving of the rows' last values (WHOLE: n_in in 16s; x's zeros are enough then) have a kernel without the code for it.  (1 x 4096 -> 4096:
 // 12.1 us with that code between the matrix instructions, each jump over it a miss.)
 constexpr uint32_t FEW_LDS = 60 * 1024;   // for x's rows
 static uint32_t few_stride(uint32_t n_in) { return (n_in + 63) / 64 * 64 + 16; }   // (+ 16: the rows of a fragment read lie on different banks)
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int t = 0; t < CT; ++t) f[h][t] = load_row16<DT_I8, WHOLE>(w[t], min(s + h, s1 - 1) * 64 + g * 16, n);
+            for (int t = 0; t < CT; ++t) f[h][t] = load_row16<DT_I8>(w[t], min(s + h, s1 - 1) * 64 + g * 16, n);
     };
     // x's units of 16 values: a row's lie on WPR waves (several a thread where it has more), RPP rows a pass
     const uint32_t units = steps * 4, wpr = min((units + 63) / 64, (uint32_t)NW), rpp = NW / wpr, my_row = wave / wpr, my_unit = (wave % wpr) * 64 + lane;
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
         if constexpr (DT == DT_I8) {
             if (s0 < s1) load_w(s0, fw);   // (a wave without a part only meets the others)
         } else {
-            const auto get = [&](uint32_t row, uint32_t u) { return load_row16<DT, WHOLE>((const char*)a.x + (uint64_t)(row0 + row) * a.ld_x * XB, u * 16, n); };
+            const auto get = [&](uint32_t row, uint32_t u) { return load_row16<DT>((const char*)a.x + (uint64_t)(row0 + row) * a.ld_x * XB, u * 16, n); };
             const bool one = rows <= rpp && units <= wpr * 64;   // one unit a thread: it stays in registers
             Raw<DT, 16> held = {};
             if (my_row < rows && my_unit < units) held = get(my_row, my_unit);
@@ -88,7 +88,8 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
                 for (uint32_t u = my_unit; u < units; u += wpr * 64) {
                     if (!one) held = get(row, u);
                     if (!WHOLE) keep_inside<DT>(held, u * 16, n);
-                    *(i4*)(lq + row * stride + u * 16) = quantize_n(held, rs);
+                    const i4 q = quantize_n(held, rs);
+                    *(i4*)(lq + row * stride + u * 16) = !WHOLE || u * 16 < n ? q : i4{0, 0, 0, 0};
                 }
             }
             __syncthreads();
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 const uint32_t k = min(s + h, s1 - 1) * 64 + g * 16, row = min(r, rows - 1);
-                if constexpr (DT == DT_I8) fx[h] = load_row16<DT_I8, WHOLE>((const char*)a.x + (uint64_t)(row0 + row) * a.ld_x, k, n);
+                if constexpr (DT == DT_I8) fx[h] = load_row16<DT_I8>((const char*)a.x + (uint64_t)(row0 + row) * a.ld_x, k, n);
                 else __builtin_memcpy(&fx[h], __builtin_assume_aligned(lq + row * stride + k, 16), 16);
             }
             if (s > s0) load_w(s, fw);
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
             for (int h = 0; h < H; ++h) {
                 if (s + h >= s1) break;
                 const uint32_t k = (s + h) * 64 + g * 16;
-                if (DT == DT_I8 && !WHOLE) keep_inside<DT_I8>(fx[h], k, n);   // (x's zeros are enough, but the weights' last pieces have to be moved)
+                if (DT == DT_I8) keep_inside<DT_I8, WHOLE>(fx[h], k, n);
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
                     if (!WHOLE) keep_inside<DT_I8>(fw[h][t], k, n);
@@ -156,7 +157,7 @@ template <int DT>
 static void linear_few(const LinearArgs& a, hipStream_t s) {
     // more workgroups than the chip holds at once: twice the channels each
     const bool many = (uint64_t)a.n_out * (a.offsets ? a.n_experts : 1) > 1024 * 16;
-    if (a.n_in % 64 == 0) many ? linear_few_of<DT, 2, true>(a, s) : linear_few_of<DT, 1, true>(a, s);
+    if (a.n_in % 16 == 0) many ? linear_few_of<DT, 2, true>(a, s) : linear_few_of<DT, 1, true>(a, s);
     else many ? linear_few_of<DT, 2, false>(a, s) : linear_few_of<DT, 1, false>(a, s);
 }
 

@@ -9,7 +9,7 @@ namespace sng {
 // their maximum with two shuffles.  The weights of up to 256 channels lie in LDS in fragment order (one linear
 // ds_read_b128 a fragment, no bank conflicts), staged once for the workgroup's rows, which belong to one expert.
 // x of type DT; KC fragments of 64 a row; NB blocks of 64 channels.  YT: y's type where every piece is a whole one (n_in in
-// 16s, n_out in 8s, y aligned to 16 bytes); -1: any sizes and places, at more registers and so fewer waves.  What hides the
+// 16s, n_out in 8s); -1: any sizes, at more registers and so fewer waves.  What hides the
 // memory's latency here is waves: under 64 registers 8 a SIMD, and small workgroups.
 template <int DT, int YT, int KC, int NB>
 __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint32_t shift) {
@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
     const RowTile tile = row_tile(a, blockIdx.x, shift);
     if (tile.begin >= tile.end) return;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n0 = blockIdx.y * (NB * 64), n = a.n_in;
-    const bool wide = WHOLE ? YT == DT_F32 : a.y_dtype == DT_F32, aligned = WHOLE || y_aligned(a);
+    const bool wide = WHOLE ? YT == DT_F32 : a.y_dtype == DT_F32;
     const auto fetch = [&](uint32_t r0, Raw<DT, 16> (&raw)[KC]) {
         const char* row = (const char*)a.x + (uint64_t)min(r0 + (lane & 15), tile.end - 1) * a.ld_x * XB;
         if (!WHOLE && n < 16)
@@ -107,22 +107,19 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
                 for (int i = 0; i < 4; ++i) v[4 * t + i] = finish(acc[i], ws[i], scale, b[i], low);
             }
             if (row >= tile.end) continue;
-            if constexpr (!WHOLE) store_block(a, row, c0, g, v, left, aligned && left >= 64);
+            if constexpr (!WHOLE) store_block(a, row, c0, g, v, left, left >= 64);
             else if constexpr (YT == DT_F32) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     const uint32_t c = channel_of(t, g, true);
-                    if (c < left) *(vec<float, 4>*)((float*)a.y + (uint64_t)row * a.ld_y + c0 + c) = vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+                    if (c < left) put_piece((float*)a.y + (uint64_t)row * a.ld_y + c0 + c, vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]});
                 }
             } else {
                 using T = std::conditional_t<YT == DT_F16, _Float16, __bf16>;
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     const uint32_t c = channel_of(2 * p, g, false);
-                    vec<T, 8> o;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = (T)v[8 * p + i];
-                    if (c < left) *(vec<T, 8>*)((T*)a.y + (uint64_t)row * a.ld_y + c0 + c) = o;
+                    if (c < left) put_piece((T*)a.y + (uint64_t)row * a.ld_y + c0 + c, to_half<T>(v + 8 * p));
                 }
             }
         }
@@ -151,8 +148,7 @@ static void linear_rows_of(const LinearArgs& a, hipStream_t s) {
 }
 template <int DT>
 static void linear_rows_by_type(const LinearArgs& a, hipStream_t s) {
-    const uint64_t y_bytes = a.y_dtype == DT_F32 ? 4 : 2;
-    const bool whole = a.n_in % 16 == 0 && a.n_out % 8 == 0 && ((uint64_t)a.y | a.ld_y * y_bytes) % 16 == 0;
+    const bool whole = a.n_in % 16 == 0 && a.n_out % 8 == 0;
     if constexpr (DT == DT_I8) {
         if (whole && a.y_dtype == DT_F16) return linear_rows_of<DT, DT_F16>(a, s);
         if (whole && a.y_dtype == DT_BF16) return linear_rows_of<DT, DT_BF16>(a, s);
