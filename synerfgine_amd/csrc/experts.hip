@@ -83,23 +83,23 @@ __global__ __launch_bounds__(NW * 64) void expert_sort_one_kernel(SortArgs a, in
     const uint32_t begin = wave * (ROUNDS * 64);
     wave_ranks<ROUNDS>(a.experts, begin, a.total, e_n, id_bits, cnt + wave * e_n, lane, key, rank);
     __syncthreads();
-    uint32_t base = 0;
-    for (uint32_t e0 = 0; e0 < e_n; e0 += NW * 64) {
-        const uint32_t e = e0 + threadIdx.x;
-        uint32_t sum = 0;
-        if (e < e_n)
-            for (int w = 0; w < NW; ++w) sum += cnt[w * e_n + e];
-        uint32_t all;
-        uint32_t at = base + block_scan<NW>(sum, wave_sums, all);
-        if (e < e_n) {
-            a.offsets[e] = (int32_t)at;
-            for (int w = 0; w < NW; ++w) {
-                const uint32_t c = cnt[w * e_n + e];
-                cnt[w * e_n + e] = at;
-                at += c;
-            }
+    // a thread's experts: a run of `per`, so that one scan over the workgroup does for all of them
+    const uint32_t per = (e_n + NW * 64 - 1) / (NW * 64), e0 = min(e_n, threadIdx.x * per), e1 = min(e_n, e0 + per);
+    uint32_t sum = 0, base;
+    for (uint32_t e = e0; e < e1; ++e)
+#pragma unroll
+        for (int w = 0; w < NW; ++w) sum += cnt[w * e_n + e];
+    uint32_t at = block_scan<NW>(sum, wave_sums, base);
+    for (uint32_t e = e0; e < e1; ++e) {
+        a.offsets[e] = (int32_t)at;
+        uint32_t c[NW];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) c[w] = cnt[w * e_n + e];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            cnt[w * e_n + e] = at;
+            at += c[w];
         }
-        base += all;
     }
     if (threadIdx.x == 0) a.offsets[e_n] = (int32_t)base;
     __syncthreads();
@@ -183,51 +183,48 @@ __global__ __launch_bounds__(1024) void expert_scan_kernel(SortArgs a, uint32_t 
 
 // The rows' order goes out through LDS: a wave's lanes hold choices of as many experts as there are, and a store of theirs
 // would touch as many lines; in the workgroup's own sorted order consecutive lanes write consecutive places.
-template <int NW>
+template <int NW, bool MANY>   // MANY: up to EXPERTS_MAX experts, in static LDS (launches take 64 KiB of the other kind)
 __global__ __launch_bounds__(NW * 64) void expert_place_kernel(SortArgs a, uint32_t blocks, int id_bits) {
-    extern __shared__ uint32_t cnt[];   // [NW][n_experts], then [n_experts]: what to add to a place in the workgroup for the place in all
+    extern __shared__ uint32_t cnt_of_call[];
+    __shared__ uint32_t cnt_of_many[MANY ? (NW + 1) * EXPERTS_MAX : 1];
+    uint32_t* const cnt = MANY ? cnt_of_many : cnt_of_call;   // [NW][n_experts], then [n_experts]: what to add to a place in the workgroup for the place in all
     __shared__ uint32_t wave_sums[NW];
     __shared__ uint32_t sorted[SORT_CHUNK];   // choice in the chunk (12 bits), expert
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t e_n = a.n_experts;
     constexpr int ROUNDS = SORT_CHUNK / (NW * 64);
     uint32_t* shift = cnt + NW * e_n;
-    uint32_t total = 0, before = 0;   // of this thread's expert: asked for long before they are wanted
-    const auto ask = [&](uint32_t e) {
-        total = e < e_n ? a.counts[(size_t)blocks * e_n + e] : 0u;
-        before = e < e_n ? a.counts[(size_t)blockIdx.x * e_n + e] : 0u;
-    };
-    ask(threadIdx.x);
+    // a thread's experts: a run of `per`, so that one scan over the workgroup does for all of them.  Their counts are asked
+    // for long before they are wanted (the first one's stay in registers).
+    const uint32_t per = (e_n + NW * 64 - 1) / (NW * 64), e0 = min(e_n, threadIdx.x * per), e1 = min(e_n, e0 + per);
+    const uint32_t* __restrict__ totals = a.counts + (size_t)blocks * e_n;
+    const uint32_t* __restrict__ befores = a.counts + (size_t)blockIdx.x * e_n;
+    const uint32_t total0 = e0 < e1 ? totals[e0] : 0u, before0 = e0 < e1 ? befores[e0] : 0u;
     for (uint32_t i = threadIdx.x; i < NW * e_n; i += NW * 64) cnt[i] = 0;
     __syncthreads();
     uint32_t key[ROUNDS], rank[ROUNDS];
     const uint32_t chunk = blockIdx.x * SORT_CHUNK, begin = chunk + wave * (ROUNDS * 64);
     wave_ranks<ROUNDS>(a.experts, begin, a.total, e_n, id_bits, cnt + wave * e_n, lane, key, rank);
     __syncthreads();
-    uint32_t base = 0, local_base = 0;
-    for (uint32_t e0 = 0; e0 < e_n; e0 += NW * 64) {
-        const uint32_t e = e0 + threadIdx.x;
-        if (e0 > 0) ask(e);
-        uint32_t c[NW], here = 0;
+    uint32_t here = 0, total = total0, base, local_base;
+    for (uint32_t e = e0; e < e1; ++e) {
+        if (e > e0) total += totals[e];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) c[w] = e < e_n ? cnt[w * e_n + e] : 0u;
+        for (int w = 0; w < NW; ++w) here += cnt[w * e_n + e];
+    }
+    uint32_t local = block_scan<NW>(here, wave_sums, local_base), first = block_scan<NW>(total, wave_sums, base);
+    for (uint32_t e = e0; e < e1; ++e) {
+        if (blockIdx.x == 0) a.offsets[e] = (int32_t)first;
+        shift[e] = first + (e > e0 ? befores[e] : before0) - local;
+        first += e > e0 ? totals[e] : total0;
+        uint32_t c[NW];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) here += c[w];
-        uint32_t all, all_here;
-        const uint32_t local = local_base + block_scan<NW>(here, wave_sums, all_here);
-        const uint32_t first = base + block_scan<NW>(total, wave_sums, all);
-        if (e < e_n) {
-            if (blockIdx.x == 0) a.offsets[e] = (int32_t)first;
-            shift[e] = first + before - local;
-            uint32_t at = local;
+        for (int w = 0; w < NW; ++w) c[w] = cnt[w * e_n + e];
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                cnt[w * e_n + e] = at;
-                at += c[w];
-            }
+        for (int w = 0; w < NW; ++w) {
+            cnt[w * e_n + e] = local;
+            local += c[w];
         }
-        base += all;
-        local_base += all_here;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[e_n] = (int32_t)base;
     __syncthreads();
@@ -251,6 +248,8 @@ void launch_expert_sort(const SortArgs& a, hipStream_t s) {
     while ((1u << id_bits) < a.n_experts) ++id_bits;
     if (a.total <= 1024 && a.n_experts <= SORT_ONE_EXPERTS)
         expert_sort_one_kernel<4, 4><<<1, 256, 4 * a.n_experts * 4, s>>>(a, id_bits);
+    else if (a.total <= 4096 && a.n_experts <= SORT_ONE_EXPERTS)
+        expert_sort_one_kernel<8, 8><<<1, 512, 8 * a.n_experts * 4, s>>>(a, id_bits);
     else if (sort_in_one(a.total, a.n_experts))
         expert_sort_one_kernel<16, 16><<<1, 1024, 16 * a.n_experts * 4, s>>>(a, id_bits);
     else {
@@ -258,10 +257,8 @@ void launch_expert_sort(const SortArgs& a, hipStream_t s) {
         const int copies = a.n_experts <= 1024 ? 4 : 1;
         expert_count_kernel<<<blocks, 256, copies * a.n_experts * 4, s>>>(a, copies);
         expert_scan_kernel<<<(a.n_experts + 63) / 64, 1024, 0, s>>>(a, blocks);
-        // (as many waves as have counters of their own in 64 KiB of LDS beside the 16 KiB of sorted choices)
-        if (a.n_experts <= 1024) expert_place_kernel<8><<<blocks, 512, 9 * a.n_experts * 4, s>>>(a, blocks, id_bits);
-        else if (a.n_experts <= 2048) expert_place_kernel<4><<<blocks, 256, 5 * a.n_experts * 4, s>>>(a, blocks, id_bits);
-        else expert_place_kernel<2><<<blocks, 128, 3 * a.n_experts * 4, s>>>(a, blocks, id_bits);
+        if (a.n_experts <= 1024) expert_place_kernel<8, false><<<blocks, 512, 9 * a.n_experts * 4, s>>>(a, blocks, id_bits);
+        else expert_place_kernel<4, true><<<blocks, 256, 0, s>>>(a, blocks, id_bits);
     }
 }
 

@@ -52,6 +52,19 @@ void check_linear(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_exper
     check_experts(n_experts);
 }
 
+// The workspace of a call whose x is brought to 8 bits before the product: the rows, padded; their scales; and where n_in is
+// no multiple of 16, the weights in rows that the tiles can take (2 bytes moved a weight, where unaligned tiles took 4 to 10
+// times the time of aligned ones)
+struct LinearLayout { uint64_t scale, w, bytes; };
+LinearLayout linear_i8_layout(uint64_t rows, uint64_t n_in, uint64_t n_out, uint64_t n_experts) {
+    LinearLayout l;
+    l.scale = rows * padded(n_in);
+    l.w = l.scale + (rows * sizeof(float) + 15) / 16 * 16;
+    l.bytes = l.w;
+    if (n_in % 16 != 0 && linear_i8_kernel((uint32_t)rows, (uint32_t)n_in, (uint32_t)n_out, (uint32_t)n_experts) == LinearKernel::Tile) l.bytes += n_experts * n_out * padded(n_in);
+    return l;
+}
+
 }  // namespace
 
 uint64_t expert_sort_workspace(uint32_t n, uint32_t k, uint32_t n_experts) {
@@ -146,7 +159,7 @@ uint64_t linear_i8_workspace(uint32_t rows, uint32_t n_in, uint32_t n_out, int32
     check_linear(rows, n_in, n_out, n_experts);
     check_type(x_dtype, true);
     if (rows == 0 || x_dtype == SNG_I8 || linear_i8_quantizes(rows, n_in, n_out, n_experts)) return 0;
-    return rows * padded(n_in) + (uint64_t)rows * sizeof(float);
+    return linear_i8_layout(rows, n_in, n_out, n_experts).bytes;
 }
 
 void linear_i8(sng_ctx* c, const sng_linear_i8_args* p, hipStream_t s) {
@@ -173,12 +186,18 @@ void linear_i8(sng_ctx* c, const sng_linear_i8_args* p, hipStream_t s) {
     l.offsets = a.d_offsets; l.n_experts = a.n_experts; l.rows = a.rows; l.n_in = a.n_in; l.n_out = a.n_out; l.y = a.d_y; l.ld_y = a.ld_y;
     l.y_dtype = a.y_dtype; l.relu = a.relu;
     if (need) {
+        const LinearLayout at = linear_i8_layout(a.rows, a.n_in, a.n_out, a.n_experts);
         const uint64_t ld = padded(a.n_in);
         int8_t* q = (int8_t*)a.d_workspace;
-        float* scale = (float*)(q + a.rows * ld);
+        float* scale = (float*)(q + at.scale);
         launch_quantize_rows(QuantArgs{a.d_x, a.ld_x, a.x_dtype, a.rows, a.n_in, (uint32_t)ld, q, ld, scale}, s);
         HIPCHK(hipGetLastError());
         l.x = q; l.ld_x = ld; l.x_dtype = SNG_I8; l.x_scale = scale;
+        if (at.bytes > at.w) {
+            launch_pad_rows(a.d_w, a.ld_w, a.n_in, (uint64_t)a.n_experts * a.n_out, (uint32_t)ld, q + at.w, s);
+            HIPCHK(hipGetLastError());
+            l.w = q + at.w; l.ld_w = ld; l.n_in = (uint32_t)ld;   // (zeros behind the rows on both sides)
+        }
     }
     launch_linear_i8(l, s);
     HIPCHK(hipGetLastError());

@@ -149,7 +149,7 @@ static uint32_t row_tiles(const LinearArgs& a, uint32_t shift) {
 }
 
 // 16 elements of a row of n >= 16 from element k on (a multiple of 16), at any alignment and without reading behind the
-// row: the row's last 16 are read where fewer are left.  keep_inside then moves those to their places and clears what lies
+// row: the row's last 16 are read where fewer are left.  inside() then moves those to their places and clears what lies
 // from n on.  Two steps, so that all of a thread's loads are on their way before it waits for the first.
 template <int DT, bool INSIDE = false>   // INSIDE: k + 16 <= n
 __device__ __forceinline__ Raw<DT, 16> load_row16(const char* __restrict__ row, uint32_t k, uint32_t n) {
@@ -158,7 +158,7 @@ __device__ __forceinline__ Raw<DT, 16> load_row16(const char* __restrict__ row, 
     return r;
 }
 template <int DT, bool WHOLE = false>   // WHOLE: n is a multiple of 16
-__device__ __forceinline__ void keep_inside(Raw<DT, 16>& r, uint32_t k, uint32_t n) {
+__device__ __forceinline__ Raw<DT, 16> inside(Raw<DT, 16> r, uint32_t k, uint32_t n) {
     constexpr int XB = bytes_of(DT), W = 4 * XB;
     if (!WHOLE && n & 15) {
         const uint32_t move = (k - min(k, n - 16)) * XB;   // bytes; 16 elements and more: nothing is left
@@ -174,6 +174,7 @@ __device__ __forceinline__ void keep_inside(Raw<DT, 16>& r, uint32_t k, uint32_t
     } else
 #pragma unroll
         for (int i = 0; i < W; ++i) r.w[i] = k >= n ? 0u : r.w[i];
+    return r;
 }
 // A whole row of n < 16
 template <int DT>
@@ -197,46 +198,52 @@ __device__ __forceinline__ i4 as_fragment(const Raw<DT_I8, 16>& r) { return i4{(
 // three lanes of its row, so a store writes 64 consecutive bytes a row: 8 channels of f16 (two accumulators), 4 of f32.
 __device__ __forceinline__ uint32_t channel_of(int t, uint32_t g, bool wide) { return wide ? t * 16 + g * 4 : (t >> 1) * 32 + g * 8 + (t & 1) * 4; }
 
-// 16 bytes of y, at any place of y's type
-template <typename V>
-__device__ __forceinline__ void put_piece(void* p, const V& v) { __builtin_memcpy(p, &v, sizeof(V)); }
+// 16 bytes of y at any place, of which `left` bytes (2 or 4 in all an element) lie inside the row
+__device__ __forceinline__ void put_piece(char* p, const i4& v, uint32_t left) {
+    if (left >= 16) __builtin_memcpy(p, &v, 16);
+    else {   // 8, 4 and 2 bytes of it: a few instructions, where a store an element is a page of them
+        if (left & 8) {
+            const vec<int, 2> lo = {v[0], v[1]};
+            __builtin_memcpy(p, &lo, 8);
+        }
+        if (left & 4) {
+            const int w = left & 8 ? v[2] : v[0];
+            __builtin_memcpy(p + (left & 8), &w, 4);
+        }
+        if (left & 2) {
+            const uint16_t h = (uint16_t)(left & 8 ? (left & 4 ? v[3] : v[2]) : (left & 4 ? v[1] : v[0]));
+            __builtin_memcpy(p + (left & 12), &h, 2);
+        }
+    }
+}
 template <typename T>
-__device__ __forceinline__ vec<T, 8> to_half(const float* v) {
+__device__ __forceinline__ i4 to_half(const float* v) {
     vec<T, 8> o;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = (T)v[i];
-    return o;
+    return __builtin_bit_cast(i4, o);
 }
-// One row's 16 channels of a 64-channel block from channel c0 on (v[4 t + i], channels as channel_of says), `left` channels
-// inside; whole: all 64 are
-__device__ __forceinline__ void store_block(const LinearArgs& a, uint32_t row, uint32_t c0, uint32_t g, const float (&v)[16], uint32_t left, bool whole) {
+// One row's 16 channels of a 64-channel block from channel c0 on (v[4 t + i], channels as channel_of says), `left` > 0 of the
+// 64 inside; YT: y's type, or -1: as a.y_dtype says
+template <int YT = -1>
+__device__ __forceinline__ void store_block(const LinearArgs& a, uint32_t row, uint32_t c0, uint32_t g, const float (&v)[16], uint32_t left) {
     const uint64_t at = (uint64_t)row * a.ld_y + c0;
-    if (whole) {
-        if (a.y_dtype == DT_F32) {
+    if (YT == DT_F32 || (YT < 0 && a.y_dtype == DT_F32)) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-                put_piece((float*)a.y + at + channel_of(t, g, true), vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]});
-        } else if (a.y_dtype == DT_F16) {
-#pragma unroll
-            for (int p = 0; p < 2; ++p) put_piece((_Float16*)a.y + at + channel_of(2 * p, g, false), to_half<_Float16>(v + 8 * p));
-        } else {
-#pragma unroll
-            for (int p = 0; p < 2; ++p) put_piece((__bf16*)a.y + at + channel_of(2 * p, g, false), to_half<__bf16>(v + 8 * p));
+        for (int t = 0; t < 4; ++t) {
+            const uint32_t c = channel_of(t, g, true);
+            const vec<float, 4> o = {v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+            if (left >= 64) __builtin_memcpy((char*)a.y + (at + c) * 4, &o, 16);   // (the same for all lanes: no look at each piece)
+            else if (c < left) put_piece((char*)a.y + (at + c) * 4, __builtin_bit_cast(i4, o), (left - c) * 4);
         }
-        return;
-    }
-    asm volatile("" : "+v"(left));   // (else the comparisons of every value's place are kept over the kernel's loop, in more registers than there are)
+    } else
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const uint32_t c = channel_of(t, g, a.y_dtype == DT_F32);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (c + i >= left) continue;
-            if (a.y_dtype == DT_F32) ((float*)a.y)[at + c + i] = v[4 * t + i];
-            else if (a.y_dtype == DT_F16) ((_Float16*)a.y)[at + c + i] = (_Float16)v[4 * t + i];
-            else ((__bf16*)a.y)[at + c + i] = (__bf16)v[4 * t + i];
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t c = channel_of(2 * p, g, false);
+            const i4 o = YT == DT_F16 || (YT < 0 && a.y_dtype == DT_F16) ? to_half<_Float16>(v + 8 * p) : to_half<__bf16>(v + 8 * p);
+            if (left >= 64) __builtin_memcpy((char*)a.y + (at + c) * 2, &o, 16);
+            else if (c < left) put_piece((char*)a.y + (at + c) * 2, o, (left - c) * 2);
         }
-    }
 }
 // A sum to its result: the row's scale last, since it has the type's whole range; low = 0 (ReLU) or -infinity.  NaN stays.
 __device__ __forceinline__ float finish(int sum, float w_scale, float x_scale, float bias, float low) {

@@ -58,6 +58,54 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
     }
 }
 
+// The same for rows at any place and of any length, to rows padded and aligned as the tiles want them: units of 16 values.
+template <int DT, int G>
+__global__ __launch_bounds__(256) void quantize_units_kernel(QuantArgs a) {
+    constexpr int XB = bytes_of(DT), C = 4;
+    __shared__ uint32_t part[4];
+    const uint32_t g = threadIdx.x % G, units = a.cols_written / 16, n = a.cols;
+    for (uint64_t r = blockIdx.x * (uint64_t)(256 / G) + threadIdx.x / G; r < a.rows; r += gridDim.x * (uint64_t)(256 / G)) {
+        const char* __restrict__ x = (const char*)a.x + r * a.ld_x * XB;
+        Raw<DT, 16> held[C];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < C; ++i) held[i] = load_row16<DT>(x, (g + i * G) * 16, n);   // (past the end: the row's last 16 again)
+#pragma unroll
+        for (int i = 0; i < C; ++i) top = max(top, top_bits(held[i]));
+        for (uint32_t u = g + C * G; u < units; u += G) top = max(top, top_bits(load_row16<DT>(x, u * 16, n)));
+#pragma unroll
+        for (int m = (G < 64 ? G : 64) / 2; m > 0; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
+        if constexpr (G == 256) {
+            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+            __syncthreads();
+            top = max(max(part[0], part[1]), max(part[2], part[3]));
+            __syncthreads();
+        }
+        const RowScale rs = row_scale(top);
+        if (g == 0) a.scale[r] = rs.scale;
+        const auto put = [&](Raw<DT, 16> v, uint32_t u) {
+            v = inside<DT>(v, u * 16, n);
+            *(i4*)(a.q + r * a.ld_q + u * 16) = quantize_n(v, rs);
+        };
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (g + i * G < units) put(held[i], g + i * G);
+        for (uint32_t u = g + C * G; u < units; u += G) put(load_row16<DT>(x, u * 16, n), u);
+    }
+}
+
+// 8-bit rows (weights) to padded and aligned ones
+__global__ __launch_bounds__(256) void pad_rows_kernel(const int8_t* __restrict__ w, uint64_t ld_w, uint32_t n, uint64_t rows, FastDiv units, int8_t* __restrict__ to) {
+    for (uint64_t b = blockIdx.x; b * (256 / 4) < rows; b += gridDim.x)   // 64 rows a workgroup
+        for (uint32_t i = threadIdx.x; i < 64 * units.d; i += 256) {
+            const uint32_t r = units.div(i), u = i - r * units.d;
+            if (b * 64 + r >= rows) break;
+            Raw<DT_I8, 16> v = load_row16<DT_I8>((const char*)w + (b * 64 + r) * ld_w, u * 16, n);
+            v = inside<DT_I8>(v, u * 16, n);
+            *(i4*)(to + ((b * 64 + r) * units.d + u) * 16) = as_fragment(v);
+        }
+}
+
 static uint32_t grid_of(uint64_t blocks) { return (uint32_t)std::min<uint64_t>(blocks, 1u << 22); }
 
 template <int DT, int PB>
@@ -75,7 +123,17 @@ static void quantize(const QuantArgs& a, hipStream_t s) {
     constexpr int XB = bytes_of(DT), N = 16 / XB;
     const bool wide = a.cols % N == 0 && ((uint64_t)a.x | (a.ld_x * XB)) % 16 == 0 && ((uint64_t)a.q | a.ld_q) % N == 0;
     if (wide) quantize_by_length<DT, 16>(a, s);
-    else quantize_by_length<DT, XB>(a, s);
+    else if (((uint64_t)a.q | a.ld_q | a.cols_written) % 16 == 0 && a.cols >= 16) {
+        const uint32_t units = a.cols_written / 16;
+        const auto blocks = [&](uint32_t g) { return grid_of(((uint64_t)a.rows * g + 255) / 256); };
+        if (units <= 64) quantize_units_kernel<DT, 16><<<blocks(16), 256, 0, s>>>(a);
+        else if (units <= 256 && a.rows >= 2048) quantize_units_kernel<DT, 64><<<blocks(64), 256, 0, s>>>(a);
+        else quantize_units_kernel<DT, 256><<<blocks(256), 256, 0, s>>>(a);
+    } else quantize_by_length<DT, XB>(a, s);
+}
+
+void launch_pad_rows(const int8_t* w, uint64_t ld_w, uint32_t n, uint64_t rows, uint32_t padded, int8_t* to, hipStream_t s) {
+    pad_rows_kernel<<<grid_of((rows + 63) / 64), 256, 0, s>>>(w, ld_w, n, rows, FastDiv(padded / 16), to);
 }
 
 void launch_quantize_rows(const QuantArgs& a, hipStream_t s) {
@@ -140,7 +198,7 @@ __global__ __launch_bounds__(256) void linear_i8_tile_kernel(LinearArgs a) {
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
             const uint32_t c = threadIdx.x + i * 256, row = c >> 3, piece = c & 7;
-            if (k0 + BK > a.n_in) keep_inside<DT_I8>(next[i], k0 + piece * 16, a.n_in);
+            if (k0 + BK > a.n_in) next[i] = inside<DT_I8>(next[i], k0 + piece * 16, a.n_in);
             *(i4*)(lds + row * BK + ((piece ^ (row < BM ? keyx(row) : key(row - BM))) * 16)) = as_fragment(next[i]);
         }
         __syncthreads();
@@ -296,7 +354,7 @@ __global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a,
         for (int q = 0; q < 16; ++q) {
             v[q] = finish(acc[q >> 2][u][q & 3], ws[q], s, b[q], lowest(a));
         }
-        store_block(a, row, c0, g, v, a.n_out - c0, c0 + 64 <= a.n_out);
+        store_block(a, row, c0, g, v, a.n_out - c0);
     }
 }
 
@@ -314,7 +372,8 @@ static void linear_stream(const LinearArgs& a, hipStream_t s) {
 
 LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
     if (n_in <= 256) return LinearKernel::Rows;
-    if (rows <= 16u * n_experts) return LinearKernel::Few;
+    // a fragment's 16 rows; by expert 12, since some have more (128 experts of 768 -> 1024: 12 rows 36 us, 34 in tiles; 8 rows 31, 33)
+    if (rows <= (n_experts == 1 ? 16u : 12u * n_experts)) return LinearKernel::Few;
     return LinearKernel::Tile;
 }
 bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
@@ -323,7 +382,7 @@ bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t 
 }
 
 void launch_linear_i8(const LinearArgs& a, hipStream_t s) {
-    switch (linear_i8_kernel(a.rows, a.n_in, a.n_out, a.n_experts)) {
+    switch (linear_i8_kernel(a.rows, a.n_in, a.n_out, a.n_experts)) {   // (n_in padded: the same one, above 256)
         case LinearKernel::Rows: launch_linear_rows(a, s); return;
         case LinearKernel::Few: launch_linear_few(a, s); return;
         case LinearKernel::Tile: break;

@@ -87,7 +87,7 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
 #pragma unroll 1
                 for (uint32_t u = my_unit; u < units; u += wpr * 64) {
                     if (!one) held = get(row, u);
-                    if (!WHOLE) keep_inside<DT>(held, u * 16, n);
+                    if (!WHOLE) held = inside<DT>(held, u * 16, n);
                     const i4 q = quantize_n(held, rs);
                     *(i4*)(lq + row * stride + u * 16) = !WHOLE || u * 16 < n ? q : i4{0, 0, 0, 0};
                 }
@@ -108,10 +108,10 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
             for (int h = 0; h < H; ++h) {
                 if (s + h >= s1) break;
                 const uint32_t k = (s + h) * 64 + g * 16;
-                if (DT == DT_I8) keep_inside<DT_I8, WHOLE>(fx[h], k, n);
+                if (DT == DT_I8) fx[h] = inside<DT_I8, WHOLE>(fx[h], k, n);
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
-                    if (!WHOLE) keep_inside<DT_I8>(fw[h][t], k, n);
+                    if (!WHOLE) fw[h][t] = inside<DT_I8>(fw[h][t], k, n);
                     acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as_fragment(fw[h][t]), as_fragment(fx[h]), acc[t], 0, 0, 0);
                 }
             }
@@ -161,10 +161,9 @@ static void linear_few(const LinearArgs& a, hipStream_t s) {
     else many ? linear_few_of<DT, 2, false>(a, s) : linear_few_of<DT, 1, false>(a, s);
 }
 
-// whether the rows of a group fit LDS: else they are brought to 8 bits before
-bool linear_few_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_experts) {
-    return std::min(16u, FEW_LDS / few_stride(n_in)) >= (n_experts == 1 ? rows : 8u);
-}
+// Whether x is brought to 8 bits by every workgroup or before, by a launch of its own: up to 32768 values an expert's rows
+// (4096 -> 4096: 8 rows 9.8 us, 16 rows 9.6 us with the launch and more without; 8192 -> 1024: 4 rows 11.5, 8 rows 12.2)
+bool linear_few_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_experts) { return (uint64_t)rows * n_in <= 32768ull * n_experts && few_stride(n_in) <= FEW_LDS / 2; }
 void launch_linear_few(const LinearArgs& a, hipStream_t s) {
     by_type(a.x_dtype, [&](auto t) { linear_few<decltype(t)::value>(a, s); });
 }

@@ -8,13 +8,13 @@ namespace sng {
 // A lane holds the 16 consecutive values of one row that the matrix instruction wants of it; the four lanes of a row share
 // their maximum with two shuffles.  The weights of up to 256 channels lie in LDS in fragment order (one linear
 // ds_read_b128 a fragment, no bank conflicts), staged once for the workgroup's rows, which belong to one expert.
-// x of type DT; KC fragments of 64 a row; NB blocks of 64 channels.  YT: y's type where every piece is a whole one (n_in in
-// 16s, n_out in 8s); -1: any sizes, at more registers and so fewer waves.  What hides the
+// x of type DT; KC fragments of 64 a row; NB blocks of 64 channels.  YT: y's type where x's pieces are whole ones (n_in in 16s);
+// -1: any n_in from 16 on and any type, at more registers and so fewer waves; -2: n_in below 16.  What hides the
 // memory's latency here is waves: under 64 registers 8 a SIMD, and small workgroups.
 template <int DT, int YT, int KC, int NB>
 __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint32_t shift) {
     constexpr int XB = bytes_of(DT);
-    constexpr bool WHOLE = YT >= 0;
+    constexpr bool WHOLE = YT >= 0, TINY = YT == -2;
     __shared__ i4 lw[NB * 4 * KC * 64];
     __shared__ __align__(16) float lscale[NB * 64], lbias[NB * 64];
     const RowTile tile = row_tile(a, blockIdx.x, shift);
@@ -23,18 +23,16 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
     const bool wide = WHOLE ? YT == DT_F32 : a.y_dtype == DT_F32;
     const auto fetch = [&](uint32_t r0, Raw<DT, 16> (&raw)[KC]) {
         const char* row = (const char*)a.x + (uint64_t)min(r0 + (lane & 15), tile.end - 1) * a.ld_x * XB;
-        if (!WHOLE && n < 16)
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) raw[kc] = load_short_row<DT>(row, kc * 64 + g * 16, n);
-        else
-#pragma unroll
-            for (int kc = 0; kc < KC; ++kc) raw[kc] = load_row16<DT>(row, kc * 64 + g * 16, n);
+        for (int kc = 0; kc < KC; ++kc) raw[kc] = TINY ? load_short_row<DT>(row, kc * 64 + g * 16, n) : load_row16<DT>(row, kc * 64 + g * 16, n);
     };
     Raw<DT, 16> raw[KC];
     uint32_t r0 = tile.begin + wave * 16;
     if (r0 < tile.end) fetch(r0, raw);
-    {
+    {   // the scales' and the first weights' loads before any of them is waited for
         const int8_t* __restrict__ w = (const int8_t*)a.w + (uint64_t)tile.expert * a.n_out * a.ld_w;
+        const uint64_t c = (uint64_t)tile.expert * a.n_out + min(n0 + threadIdx.x, a.n_out - 1);   // (past the last channel: not used)
+        const float scale = a.w_scale[c], bias = a.bias ? a.bias[c] : 0.0f;
         const auto w_row = [&](int i) {   // the channel and place in it of fragment lane i * 256 + tid
             const uint32_t f = i * 256 + threadIdx.x, t = (f >> 6) / KC & 3, nb = (f >> 6) / (4 * KC);
             return (const char*)w + (uint64_t)min(n0 + nb * 64 + channel_of(t, (f >> 2) & 3, wide) + (f & 3), a.n_out - 1) * a.ld_w;
@@ -44,24 +42,17 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
         for (int i0 = 0; i0 < NB * KC; i0 += 4) {   // (up to four loads at a time: registers)
             constexpr int I = NB * KC < 4 ? NB * KC : 4;
             Raw<DT_I8, 16> fw[I];
-            if (!WHOLE && n < 16)
 #pragma unroll
-                for (int i = 0; i < I; ++i) fw[i] = load_short_row<DT_I8>(w_row(i0 + i), w_k(i0 + i), n);
-            else {
+            for (int i = 0; i < I; ++i) fw[i] = TINY ? load_short_row<DT_I8>(w_row(i0 + i), w_k(i0 + i), n) : load_row16<DT_I8>(w_row(i0 + i), w_k(i0 + i), n);
+            if (!TINY && n != KC * 64)
 #pragma unroll
-                for (int i = 0; i < I; ++i) fw[i] = load_row16<DT_I8>(w_row(i0 + i), w_k(i0 + i), n);
-                if (n != KC * 64)
-#pragma unroll
-                    for (int i = 0; i < I; ++i) keep_inside<DT_I8, WHOLE>(fw[i], w_k(i0 + i), n);
-            }
+                for (int i = 0; i < I; ++i) fw[i] = inside<DT_I8, WHOLE>(fw[i], w_k(i0 + i), n);
 #pragma unroll
             for (int i = 0; i < I; ++i) lw[(i0 + i) * 256 + threadIdx.x] = as_fragment(fw[i]);   // (channels past the last: multiplied, not stored)
         }
         if (threadIdx.x < NB * 64) {
-            const uint32_t c = n0 + threadIdx.x;
-            const uint64_t at = (uint64_t)tile.expert * a.n_out + c;
-            lscale[threadIdx.x] = c < a.n_out ? a.w_scale[at] : 0.0f;
-            lbias[threadIdx.x] = c < a.n_out && a.bias ? a.bias[at] : 0.0f;
+            lscale[threadIdx.x] = scale;
+            lbias[threadIdx.x] = bias;
         }
     }
     __syncthreads();
@@ -71,9 +62,9 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
         const uint32_t row = r0 + (lane & 15);
         i4 q[KC];
         float scale;
-        if (n != KC * 64 && (WHOLE || n >= 16))
+        if (!TINY && n != KC * 64)
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) keep_inside<DT, WHOLE>(raw[kc], kc * 64 + g * 16, n);
+            for (int kc = 0; kc < KC; ++kc) raw[kc] = inside<DT, WHOLE>(raw[kc], kc * 64 + g * 16, n);
         if constexpr (DT == DT_I8) {
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) q[kc] = as_fragment(raw[kc]);
@@ -107,21 +98,7 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
                 for (int i = 0; i < 4; ++i) v[4 * t + i] = finish(acc[i], ws[i], scale, b[i], low);
             }
             if (row >= tile.end) continue;
-            if constexpr (!WHOLE) store_block(a, row, c0, g, v, left, left >= 64);
-            else if constexpr (YT == DT_F32) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const uint32_t c = channel_of(t, g, true);
-                    if (c < left) put_piece((float*)a.y + (uint64_t)row * a.ld_y + c0 + c, vec<float, 4>{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]});
-                }
-            } else {
-                using T = std::conditional_t<YT == DT_F16, _Float16, __bf16>;
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint32_t c = channel_of(2 * p, g, false);
-                    if (c < left) put_piece((T*)a.y + (uint64_t)row * a.ld_y + c0 + c, to_half<T>(v + 8 * p));
-                }
-            }
+            store_block<YT>(a, row, c0, g, v, left);
         }
     }
 }
@@ -132,8 +109,10 @@ static void linear_rows(const LinearArgs& a, hipStream_t s) {
     // 61.8).
     uint32_t shift = 6;
     if ((a.rows >> shift) > 2048) ++shift;
-    const uint32_t nb = a.n_out <= 64 ? 1 : a.n_out <= 128 && YT >= 0 ? 2 : 4;
-    const dim3 grid(row_tiles(a, shift), (a.n_out + nb * 64 - 1) / (nb * 64));
+    // Channels a workgroup: 64 where there are few rows (staging 256 channels of 256 weights took 7 us of a 3.5 us call);
+    // more where the rows fill the chip, since x is read and brought to 8 bits again for each of them.
+    const uint32_t tiles = row_tiles(a, shift), nb = a.n_out <= 64 || tiles < 256 ? 1 : a.n_out <= 128 && YT >= 0 ? 2 : 4;
+    const dim3 grid(tiles, (a.n_out + nb * 64 - 1) / (nb * 64));
     if (nb == 1) linear_i8_rows_kernel<DT, YT, KC, 1><<<grid, 256, 0, s>>>(a, shift);
     else if constexpr (YT >= 0) {
         if (nb == 2) linear_i8_rows_kernel<DT, YT, KC, 2><<<grid, 256, 0, s>>>(a, shift);
@@ -142,13 +121,14 @@ static void linear_rows(const LinearArgs& a, hipStream_t s) {
 }
 template <int DT, int YT>
 static void linear_rows_of(const LinearArgs& a, hipStream_t s) {
-    if (a.n_in <= 64) linear_rows<DT, YT, 1>(a, s);
+    if (a.n_in < 16) linear_rows<DT, -2, 1>(a, s);
+    else if (a.n_in <= 64) linear_rows<DT, YT, 1>(a, s);
     else if (a.n_in <= 128) linear_rows<DT, YT, 2>(a, s);
     else linear_rows<DT, YT, 4>(a, s);
 }
 template <int DT>
 static void linear_rows_by_type(const LinearArgs& a, hipStream_t s) {
-    const bool whole = a.n_in % 16 == 0 && a.n_out % 8 == 0;
+    const bool whole = a.n_in % 16 == 0;   // (n_in below 16 has its own, whatever this says)
     if constexpr (DT == DT_I8) {
         if (whole && a.y_dtype == DT_F16) return linear_rows_of<DT, DT_F16>(a, s);
         if (whole && a.y_dtype == DT_BF16) return linear_rows_of<DT, DT_BF16>(a, s);

@@ -94,6 +94,8 @@ LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint
 // whether the kernel brings x to 8 bits itself (else x has to be DT_I8)
 bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts);
 void launch_quantize_rows(const QuantArgs& a, hipStream_t s);
+// rows of n >= 16 bytes at any place to rows of `padded` (a multiple of 16), zeros behind n
+void launch_pad_rows(const int8_t* w, uint64_t ld_w, uint32_t n, uint64_t rows, uint32_t padded, int8_t* to, hipStream_t s);
 void launch_linear_i8(const LinearArgs& a, hipStream_t s);
 
 }  // namespace sng
