@@ -54,14 +54,15 @@ void check_linear(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_exper
 
 // The workspace of a call whose x is brought to 8 bits before the product: the rows, padded; their scales; and where n_in is
 // no multiple of 16, the weights in rows that the tiles can take (2 bytes moved a weight, where unaligned tiles took 4 to 10
-// times the time of aligned ones)
-struct LinearLayout { uint64_t scale, w, bytes; };
+// times the time of aligned ones); and the sums of the parts of n_in where few tiles share a long one
+struct LinearLayout { uint64_t scale, w, partial, bytes; };
 LinearLayout linear_i8_layout(uint64_t rows, uint64_t n_in, uint64_t n_out, uint64_t n_experts) {
     LinearLayout l;
     l.scale = rows * padded(n_in);
     l.w = l.scale + (rows * sizeof(float) + 15) / 16 * 16;
-    l.bytes = l.w;
-    if (n_in % 16 != 0 && linear_i8_kernel((uint32_t)rows, (uint32_t)n_in, (uint32_t)n_out, (uint32_t)n_experts) == LinearKernel::Tile) l.bytes += n_experts * n_out * padded(n_in);
+    l.partial = l.w;
+    if (n_in % 16 != 0 && linear_i8_kernel((uint32_t)rows, (uint32_t)n_in, (uint32_t)n_out, (uint32_t)n_experts) == LinearKernel::Tile) l.partial += n_experts * n_out * padded(n_in);
+    l.bytes = l.partial + linear_i8_split((uint32_t)rows, (uint32_t)n_in, (uint32_t)n_out, (uint32_t)n_experts).bytes;
     return l;
 }
 
@@ -185,6 +186,7 @@ void linear_i8(sng_ctx* c, const sng_linear_i8_args* p, hipStream_t s) {
     l.x = a.d_x; l.ld_x = a.ld_x; l.x_dtype = a.x_dtype; l.x_scale = a.d_x_scale; l.w = a.d_w; l.ld_w = a.ld_w; l.w_scale = a.d_w_scale; l.bias = a.d_bias;
     l.offsets = a.d_offsets; l.n_experts = a.n_experts; l.rows = a.rows; l.n_in = a.n_in; l.n_out = a.n_out; l.y = a.d_y; l.ld_y = a.ld_y;
     l.y_dtype = a.y_dtype; l.relu = a.relu;
+    l.kernel = linear_i8_kernel(a.rows, a.n_in, a.n_out, a.n_experts);
     if (need) {
         const LinearLayout at = linear_i8_layout(a.rows, a.n_in, a.n_out, a.n_experts);
         const uint64_t ld = padded(a.n_in);
@@ -192,8 +194,9 @@ void linear_i8(sng_ctx* c, const sng_linear_i8_args* p, hipStream_t s) {
         float* scale = (float*)(q + at.scale);
         launch_quantize_rows(QuantArgs{a.d_x, a.ld_x, a.x_dtype, a.rows, a.n_in, (uint32_t)ld, q, ld, scale}, s);
         HIPCHK(hipGetLastError());
+        l.splits = linear_i8_split(a.rows, a.n_in, a.n_out, a.n_experts).splits; l.partial = (int32_t*)(q + at.partial);
         l.x = q; l.ld_x = ld; l.x_dtype = SNG_I8; l.x_scale = scale;
-        if (at.bytes > at.w) {
+        if (at.partial > at.w) {
             launch_pad_rows(a.d_w, a.ld_w, a.n_in, (uint64_t)a.n_experts * a.n_out, (uint32_t)ld, q + at.w, s);
             HIPCHK(hipGetLastError());
             l.w = q + at.w; l.ld_w = ld; l.n_in = (uint32_t)ld;   // (zeros behind the rows on both sides)

@@ -94,16 +94,19 @@ __global__ __launch_bounds__(256) void quantize_units_kernel(QuantArgs a) {
     }
 }
 
-// 8-bit rows (weights) to padded and aligned ones
-__global__ __launch_bounds__(256) void pad_rows_kernel(const int8_t* __restrict__ w, uint64_t ld_w, uint32_t n, uint64_t rows, FastDiv units, int8_t* __restrict__ to) {
-    for (uint64_t b = blockIdx.x; b * (256 / 4) < rows; b += gridDim.x)   // 64 rows a workgroup
-        for (uint32_t i = threadIdx.x; i < 64 * units.d; i += 256) {
+// 8-bit rows (weights) to padded and aligned ones, `rows_per_block` rows a workgroup
+__global__ __launch_bounds__(256) void pad_rows_kernel(const int8_t* __restrict__ w, uint64_t ld_w, uint32_t n, uint64_t rows, FastDiv units, uint32_t rows_per_block,
+                                                       int8_t* __restrict__ to) {
+    for (uint64_t r0 = blockIdx.x * (uint64_t)rows_per_block; r0 < rows; r0 += gridDim.x * (uint64_t)rows_per_block) {
+        const uint32_t count = (uint32_t)min((uint64_t)rows_per_block, rows - r0) * units.d;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < count; i += 256) {
             const uint32_t r = units.div(i), u = i - r * units.d;
-            if (b * 64 + r >= rows) break;
-            Raw<DT_I8, 16> v = load_row16<DT_I8>((const char*)w + (b * 64 + r) * ld_w, u * 16, n);
+            Raw<DT_I8, 16> v = whole(load_odd16((const char*)w + (r0 + r) * ld_w, u * 16, n));
             v = inside<DT_I8>(v, u * 16, n);
-            *(i4*)(to + ((b * 64 + r) * units.d + u) * 16) = as_fragment(v);
+            *(i4*)(to + (r0 * units.d + i) * 16) = as_fragment(v);
         }
+    }
 }
 
 static uint32_t grid_of(uint64_t blocks) { return (uint32_t)std::min<uint64_t>(blocks, 1u << 22); }
@@ -133,7 +136,8 @@ static void quantize(const QuantArgs& a, hipStream_t s) {
 }
 
 void launch_pad_rows(const int8_t* w, uint64_t ld_w, uint32_t n, uint64_t rows, uint32_t padded, int8_t* to, hipStream_t s) {
-    pad_rows_kernel<<<grid_of((rows + 63) / 64), 256, 0, s>>>(w, ld_w, n, rows, FastDiv(padded / 16), to);
+    const uint32_t per = std::max(1u, 1024 / (padded / 16));   // 4 units a thread
+    pad_rows_kernel<<<grid_of((rows + per - 1) / per), 256, 0, s>>>(w, ld_w, n, rows, FastDiv(padded / 16), per, to);
 }
 
 void launch_quantize_rows(const QuantArgs& a, hipStream_t s) {
@@ -198,8 +202,9 @@ __global__ __launch_bounds__(256) void linear_i8_tile_kernel(LinearArgs a) {
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
             const uint32_t c = threadIdx.x + i * 256, row = c >> 3, piece = c & 7;
-            if (k0 + BK > a.n_in) next[i] = inside<DT_I8>(next[i], k0 + piece * 16, a.n_in);
-            *(i4*)(lds + row * BK + ((piece ^ (row < BM ? keyx(row) : key(row - BM))) * 16)) = as_fragment(next[i]);
+            i4 v = as_fragment(next[i]);
+            if (k0 + BK > a.n_in) v = new_bytes(v, k0 + piece * 16, a.n_in);
+            *(i4*)(lds + row * BK + ((piece ^ (row < BM ? keyx(row) : key(row - BM))) * 16)) = v;
         }
         __syncthreads();
         if (k0 + BK < a.n_in) load(k0 + BK);
@@ -258,20 +263,53 @@ __global__ __launch_bounds__(256) void linear_i8_tile_kernel(LinearArgs a) {
 // Wants n_in, both strides and both addresses in multiples of 16 bytes.
 __device__ const int8_t zeros16[16] __attribute__((aligned(16))) = {};
 
-// A wave holds BM / WR rows by 64 channels.
-template <int BM, int BN, int WR, int STAGES, bool WIDE>
+// workgroups go round the 8 dies one by one: each die gets a run of neighbouring tiles, in columns of 4 row tiles, so
+// that its cache sees the same rows and channels again
+struct TilePlace { uint32_t row, col; };
+__device__ __forceinline__ TilePlace tile_place(uint32_t id, uint32_t col_tiles, uint32_t tiles) {
+    const uint32_t group = id / (4 * col_tiles), in = id - group * 4 * col_tiles, high = min(4u, tiles / col_tiles - group * 4);
+    return {group * 4 + in % high, in / high};
+}
+// The sums of a wave's XT fragments of rows from row0 on by 64 channels from c0 on, to y
+template <int XT, bool WIDE>
+__device__ __forceinline__ void finish_tile(const LinearArgs& a, const RowTile& tile, uint32_t row0, uint32_t c0, uint32_t g, uint32_t r, const i4 (&acc)[4][XT]) {
+    if (c0 >= a.n_out) return;
+    float ws[16], b[16];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const uint32_t c = c0 + channel_of(q >> 2, g, WIDE) + (q & 3);
+        const uint64_t at = (uint64_t)tile.expert * a.n_out + min(c, a.n_out - 1);
+        ws[q] = a.w_scale[at];
+        b[q] = a.bias ? a.bias[at] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < XT; ++u) {
+        const uint32_t row = row0 + u * 16 + r;
+        if (row >= tile.end) continue;
+        const float s = a.x_scale[row];
+        float v[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) v[q] = finish(acc[q >> 2][u][q & 3], ws[q], s, b[q], lowest(a));
+        store_block(a, row, c0, g, v, a.n_out - c0);
+    }
+}
+
+// A wave holds BM / WR rows by 64 channels.  SPLIT: a workgroup takes one of a.splits runs of the steps and leaves its sums
+// in a.partial; linear_i8_join_kernel adds them.
+template <int BM, int BN, int WR, int STAGES, bool WIDE, bool SPLIT = false>
 __global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a, uint32_t col_tiles, uint32_t tiles) {
     constexpr int WC = BN / 64, WAVES = WR * WC, XT = BM / WR / 16, BK = 128, STAGE = (BM + BN) * BK;
     constexpr int LOADS = (BM + BN) / 8 / WAVES;   // each brings 8 rows of 128 bytes
     __shared__ __align__(16) int8_t lds[STAGES * STAGE];
-    // workgroups go round the 8 dies one by one: each die gets a run of neighbouring tiles, in columns of 4 row tiles, so
-    // that its cache sees the same rows and channels again
-    const uint32_t per = (tiles + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (id >= tiles) return;
-    const uint32_t row_tiles = tiles / col_tiles, group = id / (4 * col_tiles), in = id - group * 4 * col_tiles, high = min(4u, row_tiles - group * 4);
-    const RowTile tile = row_tile(a, group * 4 + in % high, BM == 256 ? 8 : BM == 128 ? 7 : 6);
+    const uint32_t all = SPLIT ? tiles * a.splits : tiles, per = (all + 7) / 8, place = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (place >= all) return;
+    const uint32_t split = SPLIT ? place / tiles : 0, id = place - split * tiles;
+    const TilePlace at = tile_place(id, col_tiles, tiles);
+    const RowTile tile = row_tile(a, at.row, BM == 256 ? 8 : BM == 128 ? 7 : 6);
     if (tile.begin >= tile.end) return;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15, n0 = in / high * BN;
+    const uint32_t all_steps = (a.n_in + BK - 1) / BK, first = SPLIT ? all_steps * split / a.splits : 0;
+    const uint32_t steps = (SPLIT ? all_steps * (split + 1) / a.splits : all_steps) - first, n_in = min(steps * BK, a.n_in - first * BK);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15, n0 = at.col * BN;
     const uint32_t wm = wave / WC * (BM / WR), wn = wave % WC * 64;
     // this lane's loads: tile rows (wave + i * WAVES) * 8 + lane / 8.  Place p of fragment row r holds piece p ^ (r / 2 & 7):
     // the 16 lanes that LDS serves at a time (0-3, 12-15, 20-23, 24-27 and so on) then cover its 64 banks
@@ -285,13 +323,13 @@ __global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a,
         const uint32_t row = (wave + i * WAVES) * 8 + row8;   // (8 rows are all of x or all of w)
         const bool of_x = (wave + i * WAVES) * 8 < BM;
         piece[i] = of_x ? piece_x : piece_w;
-        if (of_x) from[i] = (const int8_t*)a.x + (uint64_t)min(tile.begin + row, tile.end - 1) * a.ld_x + piece_x;
-        else from[i] = a.w + ((uint64_t)tile.expert * a.n_out + min(n0 + row - BM, a.n_out - 1)) * a.ld_w + piece_w;
+        if (of_x) from[i] = (const int8_t*)a.x + (uint64_t)min(tile.begin + row, tile.end - 1) * a.ld_x + first * BK + piece_x;
+        else from[i] = a.w + ((uint64_t)tile.expert * a.n_out + min(n0 + row - BM, a.n_out - 1)) * a.ld_w + first * BK + piece_w;
     }
     // (pieces past the end are zeros; steps past the last are loaded too, so that the number of loads on their way is the
     // same in every step)
     const auto load = [&](uint32_t step, int i) {
-        const int8_t* p = step * BK + piece[i] < a.n_in ? from[i] + step * BK : zeros16;
+        const int8_t* p = step * BK + piece[i] < n_in ? from[i] + step * BK : zeros16;
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
                                          (__attribute__((address_space(3))) void*)(lds + step % STAGES * STAGE + (wave + i * WAVES) * 1024), 16, 0, 0);
     };
@@ -313,7 +351,6 @@ __global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a,
     for (int t = 0; t < 4; ++t) read_w(0, 0, f[0], t);
 #pragma unroll
     for (int u = 0; u < XT; ++u) read_x(0, 0, f[0], u);
-    const uint32_t steps = (a.n_in + BK - 1) / BK;
     for (uint32_t step = 0; step < steps; ++step) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -334,28 +371,33 @@ __global__ __launch_bounds__(BN * WR) void linear_i8_stream_kernel(LinearArgs a,
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load may reach LDS after the workgroup has left it
-    const uint32_t c0 = n0 + wn;
-    if (c0 >= a.n_out) return;
-    float ws[16], b[16];
+    if constexpr (SPLIT) {
+        i4* to = (i4*)a.partial + (uint64_t)(split * tiles + id) * (4 * XT * BN * WR) + threadIdx.x;
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-        const uint32_t c = c0 + channel_of(q >> 2, g, WIDE) + (q & 3);
-        const uint64_t at = (uint64_t)tile.expert * a.n_out + min(c, a.n_out - 1);
-        ws[q] = a.w_scale[at];
-        b[q] = a.bias ? a.bias[at] : 0.0f;
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < XT; ++u) to[(t * XT + u) * BN * WR] = acc[t][u];
+    } else finish_tile<XT, WIDE>(a, tile, tile.begin + wm, n0 + wn, g, r, acc);
+}
+
+// The sums that SPLIT left, added (exact: any order is the same) and finished; a workgroup a tile, its threads as there.
+template <int BM, int BN, int WR, bool WIDE>
+__global__ __launch_bounds__(BN * WR) void linear_i8_join_kernel(LinearArgs a, uint32_t col_tiles, uint32_t tiles) {
+    constexpr int XT = BM / WR / 16, WC = BN / 64;
+    const TilePlace at = tile_place(blockIdx.x, col_tiles, tiles);
+    const RowTile tile = row_tile(a, at.row, BM == 256 ? 8 : BM == 128 ? 7 : 6);
+    if (tile.begin >= tile.end) return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    i4 acc[4][XT] = {};
+#pragma unroll 4
+    for (uint32_t split = 0; split < a.splits; ++split) {
+        const i4* from = (const i4*)a.partial + (uint64_t)(split * tiles + blockIdx.x) * (4 * XT * BN * WR) + threadIdx.x;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < XT; ++u) acc[t][u] += from[(t * XT + u) * BN * WR];
     }
-#pragma unroll
-    for (int u = 0; u < XT; ++u) {
-        const uint32_t row = tile.begin + wm + u * 16 + r;
-        if (row >= tile.end) continue;
-        const float s = a.x_scale[row];
-        float v[16];
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            v[q] = finish(acc[q >> 2][u][q & 3], ws[q], s, b[q], lowest(a));
-        }
-        store_block(a, row, c0, g, v, a.n_out - c0);
-    }
+    finish_tile<XT, WIDE>(a, tile, tile.begin + wave / WC * (BM / WR), at.col * BN + wave % WC * 64, g, r, acc);
 }
 
 template <typename T>
@@ -370,10 +412,38 @@ static void linear_stream(const LinearArgs& a, hipStream_t s) {
     else linear_i8_stream_kernel<BM, BN, WR, STAGES, false><<<grid, BN * WR, 0, s>>>(a, cols, tiles);
 }
 
+// Tiles with rows in them; by expert as if all had the same number, since the host does not know the offsets
+static uint64_t tiles_likely(const LinearArgs& a, uint32_t rows, uint32_t cols) {
+    const uint64_t e = a.offsets ? a.n_experts : 1, of_one = (a.rows + e - 1) / e;
+    return e * ((of_one + rows - 1) / rows) * ((a.n_out + cols - 1) / cols);
+}
+
+static void linear_split(const LinearArgs& a, hipStream_t s) {
+    const uint32_t cols = (a.n_out + 63) / 64, tiles = row_tiles(a, 6) * cols, grid = (tiles * a.splits + 7) / 8 * 8;
+    if (a.y_dtype == DT_F32) {
+        linear_i8_stream_kernel<64, 64, 4, 4, true, true><<<grid, 256, 0, s>>>(a, cols, tiles);
+        linear_i8_join_kernel<64, 64, 4, true><<<tiles, 256, 0, s>>>(a, cols, tiles);
+    } else {
+        linear_i8_stream_kernel<64, 64, 4, 4, false, true><<<grid, 256, 0, s>>>(a, cols, tiles);
+        linear_i8_join_kernel<64, 64, 4, false><<<tiles, 256, 0, s>>>(a, cols, tiles);
+    }
+}
+
+// Up to 128 tiles of 64 x 64 leave half of the CUs or more without one; parts of at least 4 steps, up to two workgroups a CU.  (32 x
+// 8192 -> 1024: 15.7 us of 24.8, 17 x 2092 -> 321: 14.9 of 23.7; below 16 steps the join's launch is the larger part.)
+LinearSplit linear_i8_split(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
+    const uint64_t tiles = (((uint64_t)rows >> 6) + n_experts) * ((n_out + 63) / 64), steps = (n_in + 127) / 128;
+    if (linear_i8_kernel(rows, n_in, n_out, n_experts) != LinearKernel::Tile || tiles > 128 || steps < 16) return {1, 0};
+    const uint32_t splits = (uint32_t)std::min<uint64_t>(steps / 4, 512 / tiles);
+    return {splits, splits * tiles * (64 * 64 * sizeof(int32_t))};
+}
+
 LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
-    if (n_in <= 256) return LinearKernel::Rows;
+    // above 128 the rows' registers leave few waves, and every 256 channels bring x to 8 bits again (256 -> 4096: 20000 rows
+    // 85 us, 64 in tiles; 512 rows 7.1 and 9.2; 256 -> 1024, 20000 rows 28 and 32)
+    if (n_in <= 128 || (n_in <= 256 && (n_out <= 1024 || (uint64_t)rows * n_out <= 1u << 22))) return LinearKernel::Rows;
     // a fragment's 16 rows; by expert 12, since some have more (128 experts of 768 -> 1024: 12 rows 36 us, 34 in tiles; 8 rows 31, 33)
-    if (rows <= (n_experts == 1 ? 16u : 12u * n_experts)) return LinearKernel::Few;
+    if (n_in > 256 && rows <= (n_experts == 1 ? 16u : 12u * n_experts)) return LinearKernel::Few;
     return LinearKernel::Tile;
 }
 bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
@@ -382,18 +452,21 @@ bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t 
 }
 
 void launch_linear_i8(const LinearArgs& a, hipStream_t s) {
-    switch (linear_i8_kernel(a.rows, a.n_in, a.n_out, a.n_experts)) {   // (n_in padded: the same one, above 256)
+    switch (a.kernel) {
         case LinearKernel::Rows: launch_linear_rows(a, s); return;
         case LinearKernel::Few: launch_linear_few(a, s); return;
         case LinearKernel::Tile: break;
     }
     if (((uint64_t)a.x | a.ld_x | (uint64_t)a.w | a.ld_w | a.n_in) % 16 == 0) {
-        // the largest tile that still gives most of the 256 CUs one: 256 x 256 reads each operand least often
-        const uint64_t cells = (uint64_t)a.rows * a.n_out;
-        if (cells >= 192ull * 256 * 256) linear_stream<256, 256, 2, 2>(a, s);
-        else if (cells >= 192ull * 128 * 128) linear_stream<128, 128, 2, 2>(a, s);
-        else if (cells >= 96ull * 64 * 128) linear_stream<64, 128, 2, 4>(a, s);
-        else linear_stream<64, 64, 4, 4>(a, s);
+        // (measured: 4096 -> 4096, 512 rows: 64 x 128 22 us, 128 x 128 31, 256 x 256 50; 2048 rows: 69, 45, 53; 8192: 256, 158, 130;
+        // 128 experts of 100 rows, 768 -> 1024: 73, 49, 58)
+        const uint32_t slots = 256;   // CUs: a round of workgroups of 64 x 128 and 256 x 256, half a round of 128 x 128
+        const uint64_t t128 = tiles_likely(a, 128, 128), t256 = tiles_likely(a, 256, 256);
+        if (a.splits > 1) linear_split(a, s);
+        else if (tiles_likely(a, 64, 64) <= slots / 2) linear_stream<64, 64, 4, 4>(a, s);
+        else if (tiles_likely(a, 64, 128) <= (a.offsets ? slots * 7 / 8 : slots)) linear_stream<64, 128, 2, 4>(a, s);
+        else if (t128 <= 2 * slots || t128 * 17 <= (t256 + slots - 1) / slots * slots * 40) linear_stream<128, 128, 2, 2>(a, s);
+        else linear_stream<256, 256, 2, 2>(a, s);
         return;
     }
     if (a.y_dtype == DT_F16) linear<_Float16>(a, s);

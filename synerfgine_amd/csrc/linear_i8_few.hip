@@ -10,13 +10,13 @@ namespace sng {
 // that again, which is little beside its weights.  The rows are asked for first and the first weights right behind them:
 // loads come back in their order, and the weights have the time that the rows' way to 8 bits takes.
 //
-// A call runs every instruction about once, out of a cold instruction cache: what is repeated is a loop, and sizes that
-// need no moving of the rows' last values (WHOLE: n_in in 16s; x's zeros are enough then) have a kernel without the code for it.  (1 x 4096 -> 4096:
-// 12.1 us with that code between the matrix instructions, each jump over it a miss.)
+// A call runs every instruction about once, out of a cold instruction cache: what is repeated is a loop, and the weights of
+// a row's end are taken as load_row16 gives them.  (4097 -> 4096, one row: 18 us; 20.5 us with code between the
+// matrix instructions that moves them to their places, each jump over it a miss.  ODD: weights at odd places, 10 us.)
 constexpr uint32_t FEW_LDS = 60 * 1024;   // for x's rows
 static uint32_t few_stride(uint32_t n_in) { return (n_in + 63) / 64 * 64 + 16; }   // (+ 16: the rows of a fragment read lie on different banks)
 
-template <int DT, int NW, int H, int CT, bool WHOLE>   // H fragments of 64 bytes at a time
+template <int DT, int NW, int H, int CT, bool ODD>   // H fragments of 64 bytes at a time
 __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, uint32_t group, uint32_t stride) {
     constexpr int XB = bytes_of(DT), T = NW * 64, RESULTS = CT * 256 / T > 0 ? CT * 256 / T : 1;
     extern __shared__ __align__(16) int8_t lq[];   // [group][stride]
@@ -36,11 +36,16 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
 #pragma unroll
     for (int t = 0; t < CT; ++t) w[t] = (const char*)a.w + ((uint64_t)expert * a.n_out + min(n0 + t * 16 + r, a.n_out - 1)) * a.ld_w;
     // steps past this wave's last are read as its last and not multiplied
-    const auto load_w = [&](uint32_t s, Raw<DT_I8, 16> (&f)[H][CT]) {
+    using Weights = std::conditional_t<ODD, OddBytes, Raw<DT_I8, 16>>;
+    const auto load_w = [&](uint32_t s, Weights (&f)[H][CT]) {
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int t = 0; t < CT; ++t) f[h][t] = load_row16<DT_I8>(w[t], min(s + h, s1 - 1) * 64 + g * 16, n);
+            for (int t = 0; t < CT; ++t) {
+                const uint32_t k = min(s + h, s1 - 1) * 64 + g * 16;
+                if constexpr (ODD) f[h][t] = load_odd16(w[t], k, n);
+                else f[h][t] = load_row16<DT_I8>(w[t], k, n);
+            }
     };
     // x's units of 16 values: a row's lie on WPR waves (several a thread where it has more), RPP rows a pass
     const uint32_t units = steps * 4, wpr = min((units + 63) / 64, (uint32_t)NW), rpp = NW / wpr, my_row = wave / wpr, my_unit = (wave % wpr) * 64 + lane;
@@ -55,7 +60,7 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
     }
     for (uint32_t row0 = begin; row0 < end; row0 += group) {
         const uint32_t rows = min(group, end - row0);
-        Raw<DT_I8, 16> fw[H][CT];
+        Weights fw[H][CT];
         if constexpr (DT == DT_I8) {
             if (s0 < s1) load_w(s0, fw);   // (a wave without a part only meets the others)
         } else {
@@ -87,9 +92,7 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
 #pragma unroll 1
                 for (uint32_t u = my_unit; u < units; u += wpr * 64) {
                     if (!one) held = get(row, u);
-                    if (!WHOLE) held = inside<DT>(held, u * 16, n);
-                    const i4 q = quantize_n(held, rs);
-                    *(i4*)(lq + row * stride + u * 16) = !WHOLE || u * 16 < n ? q : i4{0, 0, 0, 0};
+                    *(i4*)(lq + row * stride + u * 16) = new_bytes(quantize_n(held, rs), u * 16, n);
                 }
             }
             __syncthreads();
@@ -108,12 +111,10 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
             for (int h = 0; h < H; ++h) {
                 if (s + h >= s1) break;
                 const uint32_t k = (s + h) * 64 + g * 16;
-                if (DT == DT_I8) fx[h] = inside<DT_I8, WHOLE>(fx[h], k, n);
+                i4 x = as_fragment(fx[h]);
+                if (DT == DT_I8 && (s + h + 1) * 64 > n) x = new_bytes(x, k, n);
 #pragma unroll
-                for (int t = 0; t < CT; ++t) {
-                    if (!WHOLE) fw[h][t] = inside<DT_I8>(fw[h][t], k, n);
-                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as_fragment(fw[h][t]), as_fragment(fx[h]), acc[t], 0, 0, 0);
-                }
+                for (int t = 0; t < CT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(as_fragment(whole(fw[h][t])), x, acc[t], 0, 0, 0);
             }
         }
 #pragma unroll
@@ -145,25 +146,26 @@ __global__ __launch_bounds__(NW * 64) void linear_i8_few_kernel(LinearArgs a, ui
     }
 }
 
-template <int DT, int CT, bool WHOLE>
+template <int DT, int CT, bool ODD>
 static void linear_few_of(const LinearArgs& a, hipStream_t s) {
     const uint32_t stride = few_stride(a.n_in), group = DT == DT_I8 ? 16 : std::min(16u, FEW_LDS / stride), lds = DT == DT_I8 ? 0 : group * stride;
     const dim3 grid((a.n_out + 16 * CT - 1) / (16 * CT), a.offsets ? a.n_experts : 1);
-    if (a.n_in <= 1024) linear_i8_few_kernel<DT, 4, 4, CT, WHOLE><<<grid, 256, lds, s>>>(a, group, stride);
-    else linear_i8_few_kernel<DT, 8, (CT > 1 ? 4 : 8), CT, WHOLE><<<grid, 512, lds, s>>>(a, group, stride);
+    if (a.n_in <= 1024) linear_i8_few_kernel<DT, 4, 4, CT, ODD><<<grid, 256, lds, s>>>(a, group, stride);
+    else linear_i8_few_kernel<DT, 8, (CT > 1 ? 4 : 8), CT, ODD><<<grid, 512, lds, s>>>(a, group, stride);
 }
 
 template <int DT>
 static void linear_few(const LinearArgs& a, hipStream_t s) {
     // more workgroups than the chip holds at once: twice the channels each
-    const bool many = (uint64_t)a.n_out * (a.offsets ? a.n_experts : 1) > 1024 * 16;
-    if (a.n_in % 16 == 0) many ? linear_few_of<DT, 2, true>(a, s) : linear_few_of<DT, 1, true>(a, s);
+    const bool many = (uint64_t)a.n_out * (a.offsets ? a.n_experts : 1) > 1024 * 16, odd = ((uint64_t)a.w | a.ld_w | a.n_in) % 4 != 0;
+    if (odd) many ? linear_few_of<DT, 2, true>(a, s) : linear_few_of<DT, 1, true>(a, s);
     else many ? linear_few_of<DT, 2, false>(a, s) : linear_few_of<DT, 1, false>(a, s);
 }
 
-// Whether x is brought to 8 bits by every workgroup or before, by a launch of its own: up to 32768 values an expert's rows
-// (4096 -> 4096: 8 rows 9.8 us, 16 rows 9.6 us with the launch and more without; 8192 -> 1024: 4 rows 11.5, 8 rows 12.2)
-bool linear_few_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_experts) { return (uint64_t)rows * n_in <= 32768ull * n_experts && few_stride(n_in) <= FEW_LDS / 2; }
+// Whether x is brought to 8 bits by every workgroup or before, by a launch of its own (which costs the host 3 us too): up to
+// 24576 values an expert's rows (4096 -> 4096, f32: 6 rows 11.2 us, 12 rows 9.9 us with the launch; bf16 8.9 and 9.7; 8192 -> 1024: 2 rows 9.4, 4 rows
+// 11.7)
+bool linear_few_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_experts) { return (uint64_t)rows * n_in <= 24576ull * n_experts && few_stride(n_in) <= FEW_LDS / 2; }
 void launch_linear_few(const LinearArgs& a, hipStream_t s) {
     by_type(a.x_dtype, [&](auto t) { linear_few<decltype(t)::value>(a, s); });
 }

@@ -8,19 +8,19 @@ namespace sng {
 // A lane holds the 16 consecutive values of one row that the matrix instruction wants of it; the four lanes of a row share
 // their maximum with two shuffles.  The weights of up to 256 channels lie in LDS in fragment order (one linear
 // ds_read_b128 a fragment, no bank conflicts), staged once for the workgroup's rows, which belong to one expert.
-// x of type DT; KC fragments of 64 a row; NB blocks of 64 channels.  YT: y's type where x's pieces are whole ones (n_in in 16s);
-// -1: any n_in from 16 on and any type, at more registers and so fewer waves; -2: n_in below 16.  What hides the
+// x of type DT; KC fragments of 64 a row; NB blocks of 64 channels.  YT: y's type, or -1: any, at more registers and so fewer waves;
+// -2: any, and n_in below 16.  What hides the
 // memory's latency here is waves: under 64 registers 8 a SIMD, and small workgroups.
 template <int DT, int YT, int KC, int NB>
 __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint32_t shift) {
     constexpr int XB = bytes_of(DT);
-    constexpr bool WHOLE = YT >= 0, TINY = YT == -2;
+    constexpr bool TINY = YT == -2;
     __shared__ i4 lw[NB * 4 * KC * 64];
     __shared__ __align__(16) float lscale[NB * 64], lbias[NB * 64];
     const RowTile tile = row_tile(a, blockIdx.x, shift);
     if (tile.begin >= tile.end) return;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n0 = blockIdx.y * (NB * 64), n = a.n_in;
-    const bool wide = WHOLE ? YT == DT_F32 : a.y_dtype == DT_F32;
+    const bool wide = YT >= 0 ? YT == DT_F32 : a.y_dtype == DT_F32;
     const auto fetch = [&](uint32_t r0, Raw<DT, 16> (&raw)[KC]) {
         const char* row = (const char*)a.x + (uint64_t)min(r0 + (lane & 15), tile.end - 1) * a.ld_x * XB;
 #pragma unroll
@@ -44,9 +44,6 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
             Raw<DT_I8, 16> fw[I];
 #pragma unroll
             for (int i = 0; i < I; ++i) fw[i] = TINY ? load_short_row<DT_I8>(w_row(i0 + i), w_k(i0 + i), n) : load_row16<DT_I8>(w_row(i0 + i), w_k(i0 + i), n);
-            if (!TINY && n != KC * 64)
-#pragma unroll
-                for (int i = 0; i < I; ++i) fw[i] = inside<DT_I8, WHOLE>(fw[i], w_k(i0 + i), n);
 #pragma unroll
             for (int i = 0; i < I; ++i) lw[(i0 + i) * 256 + threadIdx.x] = as_fragment(fw[i]);   // (channels past the last: multiplied, not stored)
         }
@@ -62,9 +59,6 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
         const uint32_t row = r0 + (lane & 15);
         i4 q[KC];
         float scale;
-        if (!TINY && n != KC * 64)
-#pragma unroll
-            for (int kc = 0; kc < KC; ++kc) raw[kc] = inside<DT, WHOLE>(raw[kc], kc * 64 + g * 16, n);
         if constexpr (DT == DT_I8) {
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) q[kc] = as_fragment(raw[kc]);
@@ -79,6 +73,12 @@ __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint3
             scale = rs.scale;
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) q[kc] = quantize_n(raw[kc], rs);
+        }
+        if (!TINY && n != KC * 64) {
+            uint32_t k = g * 16;
+            asm volatile("" : "+v"(k));   // (masks made ahead of the loop would stay in registers)
+#pragma unroll
+            for (int kc = KC / 2; kc < KC; ++kc) q[kc] = new_bytes(q[kc], kc * 64 + k, n);   // (n is above KC / 2 fragments)
         }
         if (r0 + 64 < tile.end) fetch(r0 + 64, raw);   // before the stores: a wait for loads is one for the stores before them too
 #pragma unroll
@@ -128,13 +128,12 @@ static void linear_rows_of(const LinearArgs& a, hipStream_t s) {
 }
 template <int DT>
 static void linear_rows_by_type(const LinearArgs& a, hipStream_t s) {
-    const bool whole = a.n_in % 16 == 0;   // (n_in below 16 has its own, whatever this says)
     if constexpr (DT == DT_I8) {
-        if (whole && a.y_dtype == DT_F16) return linear_rows_of<DT, DT_F16>(a, s);
-        if (whole && a.y_dtype == DT_BF16) return linear_rows_of<DT, DT_BF16>(a, s);
-        if (whole) return linear_rows_of<DT, DT_F32>(a, s);
-    } else if (whole && a.y_dtype == DT) return linear_rows_of<DT, DT>(a, s);   // (a layer's output is its input's type; others: the general one)
-    linear_rows_of<DT, -1>(a, s);
+        if (a.y_dtype == DT_F16) linear_rows_of<DT, DT_F16>(a, s);
+        else if (a.y_dtype == DT_BF16) linear_rows_of<DT, DT_BF16>(a, s);
+        else linear_rows_of<DT, DT_F32>(a, s);
+    } else if (a.y_dtype == DT) linear_rows_of<DT, DT>(a, s);   // (a layer's output is its input's type; others: the general one)
+    else linear_rows_of<DT, -1>(a, s);
 }
 
 void launch_linear_rows(const LinearArgs& a, hipStream_t s) {
