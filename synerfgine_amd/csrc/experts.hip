@@ -69,7 +69,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wave_sums, 
     return before + incl - v;
 }
 
-// Everything in one workgroup: ranks, the scan over waves and experts, the plan.  One launch instead of three for the
+// Everything in one workgroup: ranks, the scan over waves and experts, the plan.  One launch instead of two or three for the
 // small calls, where launches are the time.
 template <int NW, int ROUNDS>
 __global__ __launch_bounds__(NW * 64) void expert_sort_one_kernel(SortArgs a, int id_bits) {
@@ -115,7 +115,8 @@ __global__ __launch_bounds__(NW * 64) void expert_sort_one_kernel(SortArgs a, in
     }
 }
 
-// Three launches: counts per (workgroup, expert); their exclusive sums down the workgroups; ranks and the plan.
+// Two launches or three: counts per (workgroup, expert); where they are many, their exclusive sums down the workgroups; ranks
+// and the plan.
 __global__ __launch_bounds__(256) void expert_count_kernel(SortArgs a, int copies) {
     extern __shared__ uint32_t cnt[];   // [copies][n_experts]: a wave's own counters where they fit, so that fewer adds meet
     for (uint32_t e = threadIdx.x; e < copies * a.n_experts; e += 256) cnt[e] = 0;
@@ -183,7 +184,10 @@ __global__ __launch_bounds__(1024) void expert_scan_kernel(SortArgs a, uint32_t 
 
 // The rows' order goes out through LDS: a wave's lanes hold choices of as many experts as there are, and a store of theirs
 // would touch as many lines; in the workgroup's own sorted order consecutive lanes write consecutive places.
-template <int NW, bool MANY>   // MANY: up to EXPERTS_MAX experts, in static LDS (launches take 64 KiB of the other kind)
+// MANY: up to EXPERTS_MAX experts, in static LDS (launches take 64 KiB of the other kind).  ADDS: the counts are as
+// expert_count_kernel left them, and every workgroup adds up those before its own: that is quicker than a launch while they
+// are few.
+template <int NW, bool MANY, bool ADDS>
 __global__ __launch_bounds__(NW * 64) void expert_place_kernel(SortArgs a, uint32_t blocks, int id_bits) {
     extern __shared__ uint32_t cnt_of_call[];
     __shared__ uint32_t cnt_of_many[MANY ? (NW + 1) * EXPERTS_MAX : 1];
@@ -194,18 +198,41 @@ __global__ __launch_bounds__(NW * 64) void expert_place_kernel(SortArgs a, uint3
     const uint32_t e_n = a.n_experts;
     constexpr int ROUNDS = SORT_CHUNK / (NW * 64);
     uint32_t* shift = cnt + NW * e_n;
+    uint32_t *all = shift + e_n, *before = all + e_n;   // ADDS: of each expert, in all workgroups and in those before this one
     // a thread's experts: a run of `per`, so that one scan over the workgroup does for all of them.  Their counts are asked
     // for long before they are wanted (the first one's stay in registers).
     const uint32_t per = (e_n + NW * 64 - 1) / (NW * 64), e0 = min(e_n, threadIdx.x * per), e1 = min(e_n, e0 + per);
-    const uint32_t* __restrict__ totals = a.counts + (size_t)blocks * e_n;
-    const uint32_t* __restrict__ befores = a.counts + (size_t)blockIdx.x * e_n;
-    const uint32_t total0 = e0 < e1 ? totals[e0] : 0u, before0 = e0 < e1 ? befores[e0] : 0u;
-    for (uint32_t i = threadIdx.x; i < NW * e_n; i += NW * 64) cnt[i] = 0;
+    const uint32_t* __restrict__ totals = ADDS ? all : a.counts + (size_t)blocks * e_n;
+    const uint32_t* __restrict__ befores = ADDS ? before : a.counts + (size_t)blockIdx.x * e_n;
+    uint32_t total0 = 0, before0 = 0;
+    if (!ADDS && e0 < e1) {
+        total0 = totals[e0];
+        before0 = befores[e0];
+    }
+    for (uint32_t i = threadIdx.x; i < (ADDS ? NW + 3 : NW) * e_n; i += NW * 64) cnt[i] = 0;
     __syncthreads();
+    if constexpr (ADDS) {   // consecutive threads take the experts of one workgroup's counts, as many times as there is room
+        const uint32_t width = min(1u << id_bits, (uint32_t)(NW * 64)), parts = NW * 64 / width, part = threadIdx.x / width;
+        for (uint32_t e = threadIdx.x % width; e < e_n; e += width) {
+            uint32_t sum = 0, lower = 0;
+#pragma unroll 8
+            for (uint32_t b = part; b < blocks; b += parts) {
+                const uint32_t c = a.counts[(size_t)b * e_n + e];
+                sum += c;
+                lower += b < blockIdx.x ? c : 0u;
+            }
+            atomicAdd(&all[e], sum);
+            atomicAdd(&before[e], lower);
+        }
+    }
     uint32_t key[ROUNDS], rank[ROUNDS];
     const uint32_t chunk = blockIdx.x * SORT_CHUNK, begin = chunk + wave * (ROUNDS * 64);
     wave_ranks<ROUNDS>(a.experts, begin, a.total, e_n, id_bits, cnt + wave * e_n, lane, key, rank);
     __syncthreads();
+    if (ADDS && e0 < e1) {
+        total0 = totals[e0];
+        before0 = befores[e0];
+    }
     uint32_t here = 0, total = total0, base, local_base;
     for (uint32_t e = e0; e < e1; ++e) {
         if (e > e0) total += totals[e];
@@ -243,6 +270,10 @@ __global__ __launch_bounds__(NW * 64) void expert_place_kernel(SortArgs a, uint3
 }
 static_assert(SORT_CHUNK == 4096 && EXPERTS_MAX <= 1 << 20, "a choice of the chunk and its expert share 32 bits");
 
+// (64 experts: 400000 choices, 6272 counts, 14.5 us for 15.7 with the scan's launch; 2^20 choices, 16384 counts, 20.5 for 16.8;
+// 16 experts, 2^20: 4096 counts, 13.8 for 16.1)
+constexpr uint64_t SORT_ADD_COUNTS = 1 << 13;
+
 void launch_expert_sort(const SortArgs& a, hipStream_t s) {
     int id_bits = 0;
     while ((1u << id_bits) < a.n_experts) ++id_bits;
@@ -256,9 +287,13 @@ void launch_expert_sort(const SortArgs& a, hipStream_t s) {
         const uint32_t blocks = sort_blocks(a.total);
         const int copies = a.n_experts <= 1024 ? 4 : 1;
         expert_count_kernel<<<blocks, 256, copies * a.n_experts * 4, s>>>(a, copies);
+        if (a.n_experts <= 1024 && (uint64_t)blocks * a.n_experts <= SORT_ADD_COUNTS) {
+            expert_place_kernel<8, false, true><<<blocks, 512, 11 * a.n_experts * 4, s>>>(a, blocks, id_bits);
+            return;
+        }
         expert_scan_kernel<<<(a.n_experts + 63) / 64, 1024, 0, s>>>(a, blocks);
-        if (a.n_experts <= 1024) expert_place_kernel<8, false><<<blocks, 512, 9 * a.n_experts * 4, s>>>(a, blocks, id_bits);
-        else expert_place_kernel<4, true><<<blocks, 256, 0, s>>>(a, blocks, id_bits);
+        if (a.n_experts <= 1024) expert_place_kernel<8, false, false><<<blocks, 512, 9 * a.n_experts * 4, s>>>(a, blocks, id_bits);
+        else expert_place_kernel<4, true, false><<<blocks, 256, 0, s>>>(a, blocks, id_bits);
     }
 }
 

@@ -25,7 +25,7 @@ struct FastDiv {
 
 // ---- samples by expert (experts.hip) ----------------------------------------------------------------------------
 constexpr uint32_t EXPERTS_MAX = 4096;            // a wave's counters of every expert fit 16 KiB of LDS
-constexpr uint32_t SORT_CHUNK = 4096;             // choices per workgroup of the three-launch sort
+constexpr uint32_t SORT_CHUNK = 4096;             // choices per workgroup of the sort that is not
 constexpr uint32_t SORT_ONE_MAX = 16384;          // most choices that one workgroup sorts in one launch ...
 constexpr uint32_t SORT_ONE_EXPERTS = 1024;       // ... over at most this many experts (16 waves x 4 KiB of LDS)
 constexpr uint64_t CHOICES_MAX = 1ull << 28;
