@@ -115,6 +115,8 @@ __global__ __launch_bounds__(NW * 64) void expert_sort_one_kernel(SortArgs a, in
     }
 }
 
+// Bound by launches and by the chain of steps in a workgroup, not by its 12 bytes a choice: 2^21 choices of 64 experts take
+// 5 + 5 + 13 us, 17000 take 11.
 // Two launches or three: counts per (workgroup, expert); where they are many, their exclusive sums down the workgroups; ranks
 // and the plan.
 __global__ __launch_bounds__(256) void expert_count_kernel(SortArgs a, int copies) {
@@ -328,7 +330,8 @@ template <typename V>
 __device__ __forceinline__ void put_piece(void* p, const V& v) { __builtin_memcpy(p, &v, sizeof(V)); }
 
 // Each sample's row to all its places: x is read once and in order, and a row's pieces go out together.  (The other way
-// round, rows of the sorted order gathered, reads a cache line of x for each 28-byte row: 2^20 x 2 such rows 45 us.)
+// round, rows of the sorted order gathered, reads a cache line of x for each 28-byte row: 2^20 x 2 such rows 45 us, this way
+// 29.)  Bound by memory, there by the parts of lines that its writes touch: 3.3 TB/s.
 template <typename T>   // a piece's bytes
 __global__ __launch_bounds__(256) void expert_scatter_kernel(RowsArgs a, uint32_t elem, uint32_t samples_per_block, Pieces pieces) {
     constexpr int U = 4;
@@ -378,7 +381,8 @@ void launch_expert_dispatch(const RowsArgs& a, hipStream_t s) {
 }
 
 // y[t] = sum_j w[t,j] rows[slot[t,j]], f32 in the order of j, rounded once.  The places and weights of J choices are asked
-// for together, then their J pieces, so that a thread waits twice for J choices and not twice for each.
+// for together, then their J pieces, so that a thread waits twice for J choices and not twice for each.  Bound by memory:
+// 4099 x 8 rows of 4096 bf16, 302 MB, 64 us (4.7 TB/s); 2^20 x 2 rows of 4 f16, whose places are read at random, 12.5 us (3.4).
 template <typename T, int N, int J>
 __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_t rows_per_block, Pieces pieces) {
     using V = vec<T, N>;
@@ -445,7 +449,8 @@ void launch_expert_combine(const RowsArgs& a, hipStream_t s) {
 
 // The gradient of the combine, sample by sample: G threads share one sample, so dy's row is read once for all its
 // choices, each row of the sorted order is read and its gradient written once, and a choice's weight gradient is one
-// reduction over the G threads (f32 sums, one per thread, then a tree).
+// reduction over the G threads (f32 sums, one per thread, then a tree).  Bound by memory: 16384 x 2 rows of 2048 f16,
+// 336 MB, 63 us (5.3 TB/s, a large copy's rate).
 template <typename T, int N, int G>
 __global__ __launch_bounds__(256) void expert_combine_backward_kernel(RowsArgs a) {
     using V = vec<T, N>;
