@@ -382,7 +382,7 @@ void launch_expert_dispatch(const RowsArgs& a, hipStream_t s) {
 
 // y[t] = sum_j w[t,j] rows[slot[t,j]], f32 in the order of j, rounded once.  The places and weights of J choices are asked
 // for together, then their J pieces, so that a thread waits twice for J choices and not twice for each.  Bound by memory:
-// 4099 x 8 rows of 4096 bf16, 302 MB, 64 us (4.7 TB/s); 2^20 x 2 rows of 4 f16, whose places are read at random, 12.5 us (3.4).
+// 4099 x 8 rows of 4096 bf16, 302 MB, 64 us (4.7 TB/s); 2^20 x 2 rows of 4 f16, 42 MB, 9.0 us (4.7).
 template <typename T, int N, int J>
 __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_t rows_per_block, Pieces pieces) {
     using V = vec<T, N>;
@@ -390,6 +390,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
     const T* __restrict__ src = (const T*)a.src;
     T* __restrict__ dst = (T*)a.dst;
     for (uint32_t b = blockIdx.x; b * (uint64_t)rows_per_block < a.n; b += gridDim.x)
+#pragma unroll (J <= 2 ? 2 : 1)
         for (uint32_t i = threadIdx.x, t0 = b * rows_per_block, rows = min(rows_per_block, a.n - t0); i < rows * pieces.count.d; i += 256) {
             const uint32_t r = pieces.count.div(i), c = pieces.start(i - r * pieces.count.d);
             const uint32_t first = (t0 + r) * a.k;
@@ -398,12 +399,19 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
                 uint32_t at[J];
                 float w[J];
                 V v[J];
+                if constexpr (J <= 2) {   // all of a sample's choices
+                    __builtin_memcpy(at, a.slot + first, sizeof(at));
+                    if (a.weights) __builtin_memcpy(w, a.weights + first, sizeof(w));
+                    else
 #pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const uint32_t i = first + min(j0 + j, a.k - 1);
-                    at[j] = (uint32_t)a.slot[i];
-                    w[j] = a.weights ? a.weights[i] : 1.0f;
-                }
+                        for (int j = 0; j < J; ++j) w[j] = 1.0f;
+                } else
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const uint32_t i = first + min(j0 + j, a.k - 1);
+                        at[j] = (uint32_t)a.slot[i];
+                        w[j] = a.weights ? a.weights[i] : 1.0f;
+                    }
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     if (j0 + j >= a.k) at[j] = total;
@@ -425,7 +433,10 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
 template <typename T, int N>
 static void combine(const RowsArgs& a, hipStream_t s) {
     const Pieces pieces(a.d, N);
-    const uint32_t rows = std::max(1u, 256u / pieces.count.d), grid = grid_of((a.n + rows - 1) / rows);
+    // four pieces a thread where there is work for the chip in that, and a sample's choices are one load (2^20 x 2 rows of 4 f16
+    // 9.0 us, one piece a thread 11.9; 2^18 x 4 rows 6.1 and 5.3, 2^18 x 2 rows of 128 28.2 and 27.6)
+    const bool four = a.k <= 2 && pieces.count.d <= 8 && (uint64_t)a.n * pieces.count.d >= 1u << 19;
+    const uint32_t rows = std::max(1u, (four ? 1024u : 256u) / pieces.count.d), grid = grid_of((a.n + rows - 1) / rows);
     if (a.k == 1) expert_combine_kernel<T, N, 1><<<grid, 256, 0, s>>>(a, rows, pieces);
     else if (a.k == 2) expert_combine_kernel<T, N, 2><<<grid, 256, 0, s>>>(a, rows, pieces);
     else if (a.k <= 4) expert_combine_kernel<T, N, 4><<<grid, 256, 0, s>>>(a, rows, pieces);

@@ -62,3 +62,20 @@ def test_row_lengths(tb, dtype, skew):
         err = 2.0 ** -24 * np.abs(want_r)
         assert (np.abs(got_r - want_r) <= err + R.half_step(dtype) * (np.abs(want_r) + err) + R.TINY[dtype])[live].all(), d
         assert (np.abs(got_w - want_w) <= d * 2.0 ** -24 * size * 1.01).all(), d
+
+
+@pytest.mark.parametrize("n,k,d,dtype", [(600001, 2, 4, 0), (600001, 1, 3, 2), (110001, 2, 33, 1), (262147, 1, 15, 0)])
+def test_combine_many_samples(tb, n, k, d, dtype):
+    """More samples than workgroups at a time: several pieces a thread"""
+    rng = np.random.default_rng([n, k, d])
+    ids = rng.integers(-1, 8, (n, k)).astype(np.int32)
+    _, _, slot = R.plan(ids, 8)
+    rows = torch.from_numpy(rng.normal(size=(n * k, d)).astype(np.float32)).to(R.TORCH[dtype])
+    w = rng.normal(size=(n, k)).astype(np.float32)
+    g, gw, gs = Guarded((n * k, d), rows.dtype, fill=rows), Guarded((n * k,), torch.float32, fill=w), Guarded((n * k,), torch.int32, fill=slot)
+    for weights in (w, None):
+        y = Guarded((n, d), rows.dtype)
+        tb.expert_combine(g.ptr, dtype, d, d, 0 if weights is None else gw.ptr, gs.ptr, n, k, y.ptr, d)
+        want, size = R.combine(_np(rows), weights, slot)
+        sums = k * 2.0 ** -24 * size * 1.01
+        assert (np.abs(y.get() - want) <= sums + R.half_step(dtype) * (np.abs(want) + sums) + R.TINY[dtype]).all()
