@@ -331,8 +331,8 @@ __device__ __forceinline__ void put_piece(void* p, const V& v) { __builtin_memcp
 
 // Each sample's row to all its places: x is read once and in order, and a row's pieces go out together.  (The other way
 // round, rows of the sorted order gathered, reads a cache line of x for each 28-byte row: 2^20 x 2 such rows 45 us, this way
-// 29.)  Bound by memory, there by the parts of lines that its writes touch: 3.3 TB/s.
-template <typename T>   // a piece's bytes
+// 23.)  Bound by memory, there by the parts of lines that its writes touch: 4.1 TB/s.
+template <typename T, int K>   // a piece's bytes; K > 0: k, whose places are asked for together with the pieces
 __global__ __launch_bounds__(256) void expert_scatter_kernel(RowsArgs a, uint32_t elem, uint32_t samples_per_block, Pieces pieces) {
     constexpr int U = 4;
     const uint32_t total = a.n * a.k;
@@ -343,20 +343,30 @@ __global__ __launch_bounds__(256) void expert_scatter_kernel(RowsArgs a, uint32_
         for (uint32_t i0 = threadIdx.x; i0 < count; i0 += 256 * U) {
             uint32_t t[U], c[U];
             T v[U];
+            uint32_t places[U][K ? K : 1];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t i = min(i0 + u * 256, count - 1);
                 t[u] = pieces.count.div(i);
                 c[u] = pieces.start(i - t[u] * pieces.count.d);
                 v[u] = get_piece<T>(x + ((t0 + t[u]) * a.ld_src + c[u]) * elem);
+                if constexpr (K > 0) __builtin_memcpy(places[u], a.slot + (t0 + t[u]) * K, sizeof(places[u]));
             }
-            for (uint32_t j = 0; j < a.k; ++j) {
-                uint32_t to[U];
+            if constexpr (K > 0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) to[u] = (uint32_t)a.slot[(t0 + t[u]) * a.k + j];
+                for (int j = 0; j < K; ++j)
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (to[u] < total && i0 + u * 256 < count) put_piece(out + ((uint64_t)to[u] * a.ld_dst + c[u]) * elem, v[u]);
+                    for (int u = 0; u < U; ++u)
+                        if (places[u][j] < total && i0 + u * 256 < count) put_piece(out + ((uint64_t)places[u][j] * a.ld_dst + c[u]) * elem, v[u]);
+            } else {
+                for (uint32_t j = 0; j < a.k; ++j) {
+                    uint32_t to[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) to[u] = (uint32_t)a.slot[(t0 + t[u]) * a.k + j];
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (to[u] < total && i0 + u * 256 < count) put_piece(out + ((uint64_t)to[u] * a.ld_dst + c[u]) * elem, v[u]);
+                }
             }
         }
     }
@@ -365,8 +375,13 @@ __global__ __launch_bounds__(256) void expert_scatter_kernel(RowsArgs a, uint32_
 template <typename T>
 static void scatter(const RowsArgs& a, uint32_t elem, hipStream_t s) {
     const Pieces pieces(a.d, sizeof(T) / elem);
-    const uint32_t samples = std::max(1u, 1024u / pieces.count.d);
-    expert_scatter_kernel<T><<<grid_of((a.n + samples - 1) / samples), 256, 0, s>>>(a, elem, samples, pieces);
+    // Rows of half a line and less: one workgroup a CU, with a run of samples each, so that the parts of a line that its steps
+    // write one after the other meet in the die's cache.  (2^20 x 2 rows of 28 bytes 23 us, 27 in as many workgroups as fit; 2^18
+    // x 4 rows 11.8 and 17.0; rows of 252 bytes 37.0 and 35.8.)
+    const uint32_t few = a.d * elem <= 64 ? (a.n + 255) / 256 : 1, samples = std::max(std::max(1u, 1024u / pieces.count.d), few);
+    const uint32_t grid = grid_of((a.n + samples - 1) / samples);
+    if (a.k == 2) expert_scatter_kernel<T, 2><<<grid, 256, 0, s>>>(a, elem, samples, pieces);
+    else expert_scatter_kernel<T, 0><<<grid, 256, 0, s>>>(a, elem, samples, pieces);
 }
 
 void launch_expert_dispatch(const RowsArgs& a, hipStream_t s) {
@@ -399,7 +414,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
                 uint32_t at[J];
                 float w[J];
                 V v[J];
-                if constexpr (J <= 2) {   // all of a sample's choices
+                if (J <= 2 || a.k == J) {   // all of a sample's choices in one load (2^18 x 8 rows of 8 f16 14.4 us, one by one 17.1)
                     __builtin_memcpy(at, a.slot + first, sizeof(at));
                     if (a.weights) __builtin_memcpy(w, a.weights + first, sizeof(w));
                     else

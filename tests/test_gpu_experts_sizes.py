@@ -79,3 +79,19 @@ def test_combine_many_samples(tb, n, k, d, dtype):
         want, size = R.combine(_np(rows), weights, slot)
         sums = k * 2.0 ** -24 * size * 1.01
         assert (np.abs(y.get() - want) <= sums + R.half_step(dtype) * (np.abs(want) + sums) + R.TINY[dtype]).all()
+
+
+@pytest.mark.parametrize("n,k,d,dtype", [(300007, 2, 7, 2), (300007, 3, 5, 0), (300007, 1, 40, 3), (200001, 2, 33, 1)])
+def test_dispatch_many_samples(tb, n, k, d, dtype):
+    """More samples than one step of every workgroup takes, in short rows and in longer ones"""
+    rng = np.random.default_rng([n, k, d])
+    ids = rng.integers(-1, 70, (n, k)).astype(np.int32)
+    _, order, slot = R.plan(ids, 70)
+    x = torch.from_numpy(rng.integers(-128, 128, (n, d)).astype(np.int8)) if dtype == 3 else _rows(rng, n, d, dtype)
+    gx, go, gs = Guarded((n, d), x.dtype, fill=x), Guarded((n * k,), torch.int32, fill=order), Guarded((n * k,), torch.int32, fill=slot)
+    out = Guarded((n * k, d), x.dtype)
+    tb.expert_dispatch(gx.ptr, dtype, d, d, go.ptr, gs.ptr, n, k, out.ptr, d)
+    want = np.full((n * k, d), 77, np.float32)
+    kept = np.flatnonzero(order >= 0)
+    want[kept] = _np(x)[order[kept] // k]
+    assert np.array_equal(out.get().astype(np.float32), want)
