@@ -12,8 +12,9 @@ namespace sng {
 // loads come back in their order, and the weights have the time that the rows' way to 8 bits takes.
 //
 // A call runs every instruction about once, out of a cold instruction cache: what is repeated is a loop, and the weights of
-// a row's end are taken as load_row16 gives them.  (4097 -> 4096, one row: 18 us; 20.5 us with code between the
-// matrix instructions that moves them to their places, each jump over it a miss.  ODD: weights at odd places, 10 us.)
+// a row's end are taken as load_row16 gives them.  (4097 -> 4096, one row, 8 waves: 18 us; 20.5 us with code between
+// the matrix instructions that moves them to their places, each jump over it a miss.  ODD: weights at odd places, 10 us;
+// with 16 waves 8.7.)
 constexpr uint32_t FEW_LDS = 60 * 1024;   // for x's rows
 static uint32_t few_stride(uint32_t n_in) { return (n_in + 63) / 64 * 64 + 16; }   // (+ 16: the rows of a fragment read lie on different banks)
 
@@ -155,6 +156,8 @@ static void linear_few_of(const LinearArgs& a, hipStream_t s) {
     // 5.0 with 4 waves; 16 experts of 1024 -> 2048, 4 rows each: 9.5 and 8.6)
     if (a.n_in <= 1024 && CT > 1) linear_i8_few_kernel<DT, 4, 4, CT, ODD><<<grid, 256, lds, s>>>(a, group, stride);
     else if (a.n_in <= 1024) linear_i8_few_kernel<DT, 8, 2, CT, ODD><<<grid, 512, lds, s>>>(a, group, stride);
+    // longer ones: 16 waves where every workgroup has a CU of its own (8192 -> 1024: a row 6.8 us, 7.8 with 8; 2048 -> 8192: 7.1 and 6.8)
+    else if (CT == 1 && grid.x * grid.y <= 256) linear_i8_few_kernel<DT, 16, 4, 1, ODD><<<grid, 1024, lds, s>>>(a, group, stride);
     else linear_i8_few_kernel<DT, 8, (CT > 1 ? 4 : 8), CT, ODD><<<grid, 512, lds, s>>>(a, group, stride);
 }
 
@@ -167,8 +170,8 @@ static void linear_few(const LinearArgs& a, hipStream_t s) {
 }
 
 // Whether x is brought to 8 bits by every workgroup or before, by a launch of its own (which costs the host 3 us too): up to
-// 24576 values an expert's rows (4096 -> 4096, f32: 6 rows 11.2 us, 12 rows 9.9 us with the launch; bf16 8.9 and 9.7; 8192 -> 1024: 2 rows 9.4, 4 rows
-// 11.7)
+// 24576 values an expert's rows (4096 -> 4096, f32: 5 rows 9.9 us, 8 rows 8.9 us with the launch; bf16: 6 rows 7.7, 8 rows 9.0;
+// 8192 -> 1024, bf16: 2 rows 8.0, 4 rows 10.6)
 bool linear_few_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_experts) { return (uint64_t)rows * n_in <= 24576ull * n_experts && few_stride(n_in) <= FEW_LDS / 2; }
 void launch_linear_few(const LinearArgs& a, hipStream_t s) {
     by_type(a.x_dtype, [&](auto t) { linear_few<decltype(t)::value>(a, s); });
