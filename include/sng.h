@@ -172,7 +172,8 @@ int sng_sh_encode(sng_ctx* ctx, const float* d_coords, uint32_t stride_floats, u
  * Device arrays in, device arrays out, enqueued on hip_stream on the context's device; nothing is allocated, kept
  * between calls or synchronised, so a call can be captured into a graph.  A workspace belongs to the call that it is
  * given to until that call has run on its stream: calls that may run at the same time (other streams, graphs) need one
- * each.  Buffers of a call must not overlap.  ld_*: elements from one row to the next, at least the row's length. */
+ * each.  Buffers of a call must not overlap, and what writes them on another stream has to be waited for on hip_stream.
+ * ld_*: elements from one row to the next, at least the row's length. */
 enum { SNG_F16 = 0, SNG_BF16 = 1, SNG_F32 = 2, SNG_I8 = 3 };   /* element types */
 /* d_experts [n][k]: choice i = t * k + j sends sample t to an expert; an id outside [0, n_experts) drops the choice
  * (a sample outside every block).  Out: d_offsets [n_experts + 1], the rows before each expert; d_slot [n][k], the row
