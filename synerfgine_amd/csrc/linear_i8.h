@@ -92,7 +92,8 @@ __device__ __forceinline__ float element(const Raw<DT, N>& r, int i) {
     return DT == DT_BF16 ? __builtin_bit_cast(float, h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
 
-// N values of a row to N bytes (a row that is not finite: anything)
+// N values of a row to N bytes (a row that is not finite: anything; a product's NaN scale hides it, where q itself is the
+// result the caller puts zeros)
 template <int DT, int N>
 __device__ __forceinline__ vec<int, N / 4> quantize_n(const Raw<DT, N>& r, const RowScale& rs) {
     float near = 0.0f;

@@ -86,7 +86,9 @@ __global__ __launch_bounds__(256) void quantize_units_kernel(QuantArgs a) {
         if (g == 0) a.scale[r] = rs.scale;
         const auto put = [&](Raw<DT, 16> v, uint32_t u) {
             v = inside<DT>(v, u * 16, n);
-            *(i4*)(a.q + r * a.ld_q + u * 16) = quantize_n(v, rs);
+            i4 q = quantize_n(v, rs);
+            if (!rs.finite) q = i4{0, 0, 0, 0};
+            *(i4*)(a.q + r * a.ld_q + u * 16) = q;
         };
 #pragma unroll
         for (int i = 0; i < C; ++i)
