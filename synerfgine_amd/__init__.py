@@ -11,6 +11,7 @@ All compute runs in the HIP kernels of libsng_hip.so; nothing here falls back
 to the CPU.
 """
 import ctypes
+import struct
 
 import numpy as np
 
@@ -20,6 +21,15 @@ from ._lib import SngError, check
 __all__ = ["Testbed", "Engine", "FrameResult", "SngError", "device_count", "F16", "BF16", "F32", "I8"]
 
 F16, BF16, F32, I8 = 0, 1, 2, 3   # element types (SNG_F16 ...)
+
+
+# Numbers that do not fit their C arguments would lose their high bits in ctypes: these raise struct.error for them
+_u32 = {n: struct.Struct("=%dI" % n).pack for n in (3, 5, 6, 7, 9)}
+_u64 = struct.Struct("=Q").pack
+
+
+def _too_large(error):
+    return SngError("a size, stride or type is not a whole number of 0 to 2^32 - 1, or the workspace's size of 0 to 2^64 - 1: %s" % error)
 
 
 def device_count():
@@ -168,6 +178,10 @@ class Testbed:
     # Device pointers in and out; types F16, BF16, F32 (I8); ld: elements from one row to the next; a pointer 0 is NULL.
     def expert_sort_workspace(self, n, k, n_experts):
         """Bytes of workspace that expert_sort needs (0 for small calls)."""
+        try:
+            _u32[3](n, k, n_experts)
+        except struct.error as error:
+            raise _too_large(error) from None
         size = ctypes.c_uint64()
         check(self._lib.sng_expert_sort_workspace(n, k, n_experts, ctypes.byref(size)))
         return size.value
@@ -175,31 +189,60 @@ class Testbed:
     def expert_sort(self, d_experts, n, k, n_experts, d_offsets, d_order, d_slot, d_workspace=0, workspace_bytes=0, stream=0):
         """Expert ids int32 [n][k] -> the plan: offsets [n_experts + 1], order [n * k], slot [n][k] (all int32).  Ids outside
         [0, n_experts) drop their choice; an expert's rows keep the order of their choices."""
+        try:
+            _u32[3](n, k, n_experts)
+            _u64(workspace_bytes)
+        except struct.error as error:
+            raise _too_large(error) from None
         check(self._lib.sng_expert_sort(self.ctx, d_experts, n, k, n_experts, d_offsets, d_order, d_slot, d_workspace, workspace_bytes, stream))
 
     def expert_dispatch(self, d_x, dtype, d, ld_x, d_order, d_slot, n, k, d_rows, ld_rows, stream=0):
         """Rows of x [n][d] in the experts' order; rows of no choice stay as they are.  Any type."""
+        try:
+            _u32[6](dtype, d, ld_x, n, k, ld_rows)
+        except struct.error as error:
+            raise _too_large(error) from None
         check(self._lib.sng_expert_dispatch(self.ctx, d_x, dtype, d, ld_x, d_order, d_slot, n, k, d_rows, ld_rows, stream))
 
     def expert_dispatch_backward(self, d_drows, dtype, d, ld_drows, d_slot, n, k, d_dx, ld_dx, stream=0):
         """The dispatch's gradient: each sample's rows added up (the combine without weights)."""
+        try:
+            _u32[6](dtype, d, ld_drows, n, k, ld_dx)
+        except struct.error as error:
+            raise _too_large(error) from None
         check(self._lib.sng_expert_combine(self.ctx, d_drows, dtype, d, ld_drows, None, d_slot, n, k, d_dx, ld_dx, stream))
 
     def expert_combine(self, d_rows, dtype, d, ld_rows, d_weights, d_slot, n, k, d_y, ld_y, stream=0):
         """y[t] = the sum of t's rows times their weights f32 [n][k] (0: ones), in f32, rounded once."""
+        try:
+            _u32[6](dtype, d, ld_rows, n, k, ld_y)
+        except struct.error as error:
+            raise _too_large(error) from None
         check(self._lib.sng_expert_combine(self.ctx, d_rows, dtype, d, ld_rows, d_weights, d_slot, n, k, d_y, ld_y, stream))
 
     def expert_combine_backward(self, d_dy, ld_dy, d_rows, ld_rows, dtype, d, d_weights, d_slot, n, k, d_drows, ld_drows, d_dweights, stream=0):
         """The combine's gradients for the rows and for the weights (f32 [n][k]); either may be 0 (not wanted)."""
+        try:
+            _u32[7](ld_dy, ld_rows, dtype, d, n, k, ld_drows)
+        except struct.error as error:
+            raise _too_large(error) from None
         check(self._lib.sng_expert_combine_backward(self.ctx, d_dy, ld_dy, d_rows, ld_rows, dtype, d, d_weights, d_slot, n, k, d_drows, ld_drows,
                                                     d_dweights, stream))
 
     def quantize_rows_i8(self, d_x, dtype, rows, cols, ld_x, d_q, ld_q, d_scale, stream=0):
         """Rows to 8 bits with a scale each: a layer's weights [n_out][n_in], or its input."""
+        try:
+            _u32[5](dtype, rows, cols, ld_x, ld_q)
+        except struct.error as error:
+            raise _too_large(error) from None
         check(self._lib.sng_quantize_rows_i8(self.ctx, d_x, dtype, rows, cols, ld_x, d_q, ld_q, d_scale, stream))
 
     def linear_i8_workspace(self, rows, n_in, n_out, x_dtype, n_experts=1):
         """Bytes of workspace that linear_i8 needs (0 where it quantises in registers, or x is I8 already)."""
+        try:
+            _u32[5](rows, n_in, n_out, x_dtype, n_experts)
+        except struct.error as error:
+            raise _too_large(error) from None
         size = ctypes.c_uint64()
         check(self._lib.sng_linear_i8_workspace(rows, n_in, n_out, x_dtype, n_experts, ctypes.byref(size)))
         return size.value
@@ -208,6 +251,11 @@ class Testbed:
                   n_experts=1, d_workspace=0, workspace_bytes=0, stream=0):
         """The linear layer in 8-bit integers: y = act((q w^T) * x_scale * w_scale + bias).  x F16 / BF16 / F32 is brought to 8
         bits within the call; I8 comes with d_x_scale.  d_offsets (expert_sort's): one matrix for each expert's rows."""
+        try:
+            _u32[9](x_dtype, rows, n_in, ld_x, ld_w, n_out, y_dtype, ld_y, n_experts)
+            _u64(workspace_bytes)
+        except struct.error as error:
+            raise _too_large(error) from None
         args = _lib.sng_linear_i8_args(d_x, d_x_scale, d_w, d_w_scale, d_bias, d_offsets, d_y, d_workspace, workspace_bytes, ld_x, ld_w, ld_y, rows, n_in,
                                        n_out, n_experts, x_dtype, y_dtype, 1 if relu else 0, 0)
         check(self._lib.sng_linear_i8(self.ctx, ctypes.byref(args), stream))
