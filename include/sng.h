@@ -172,7 +172,9 @@ int sng_sh_encode(sng_ctx* ctx, const float* d_coords, uint32_t stride_floats, u
  * Device arrays in, device arrays out, enqueued on hip_stream on the context's device; nothing is allocated, kept
  * between calls or synchronised, so a call can be captured into a graph.  A workspace belongs to the call that it is
  * given to until that call has run on its stream: calls that may run at the same time (other streams, graphs) need one
- * each.  Buffers of a call must not overlap, and what writes them on another stream has to be waited for on hip_stream.
+ * each.  Buffers of a call must not overlap.  hip_stream has to wait for all earlier work on other streams that reads or
+ * writes the memory of the call's inputs, outputs or workspace, also for work that used that memory before they were
+ * there: a caching allocator hands a freed block out again while the stream that it was freed on still works in it.
  * ld_*: elements from one row to the next, at least the row's length. */
 enum { SNG_F16 = 0, SNG_BF16 = 1, SNG_F32 = 2, SNG_I8 = 3 };   /* element types */
 /* d_experts [n][k]: choice i = t * k + j sends sample t to an expert; an id outside [0, n_experts) drops the choice

@@ -176,6 +176,7 @@ class Testbed:
 
     # ---- operators for a field made of several experts (include/sng.h) ----------------
     # Device pointers in and out; types F16, BF16, F32 (I8); ld: elements from one row to the next; a pointer 0 is NULL.
+    # stream has to wait for earlier work of other streams on the memory of inputs, outputs and workspaces.
     def expert_sort_workspace(self, n, k, n_experts):
         """Bytes of workspace that expert_sort needs (0 for small calls)."""
         try:
