@@ -419,12 +419,6 @@ static void linear_stream(const LinearArgs& a, hipStream_t s) {
     else linear_i8_stream_kernel<BM, BN, WR, STAGES, false><<<grid, BN * WR, 0, s>>>(a, cols, tiles);
 }
 
-// Tiles with rows in them; by expert as if all had the same number, since the host does not know the offsets
-static uint64_t tiles_likely(const LinearArgs& a, uint32_t rows, uint32_t cols) {
-    const uint64_t e = a.offsets ? a.n_experts : 1, of_one = (a.rows + e - 1) / e;
-    return e * ((of_one + rows - 1) / rows) * ((a.n_out + cols - 1) / cols);
-}
-
 static void linear_split(const LinearArgs& a, hipStream_t s) {
     const uint32_t cols = (a.n_out + 63) / 64, tiles = row_tiles(a, 6) * cols, grid = (tiles * a.splits + 7) / 8 * 8;
     if (a.y_dtype == DT_F32) {
@@ -436,23 +430,6 @@ static void linear_split(const LinearArgs& a, hipStream_t s) {
     }
 }
 
-// Up to 128 tiles of 64 x 64 leave half of the CUs or more without one; parts of at least 4 steps, up to two workgroups a CU.  (32 x
-// 8192 -> 1024: 15.7 us of 24.8, 17 x 2092 -> 321: 14.9 of 23.7; below 16 steps the join's launch is the larger part.)
-LinearSplit linear_i8_split(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
-    const uint64_t tiles = (((uint64_t)rows >> 6) + n_experts) * ((n_out + 63) / 64), steps = (n_in + 127) / 128;
-    if (linear_i8_kernel(rows, n_in, n_out, n_experts) != LinearKernel::Tile || tiles > 128 || steps < 16) return {1, 0};
-    const uint32_t splits = (uint32_t)std::min<uint64_t>(steps / 4, 512 / tiles);
-    return {splits, splits * tiles * (64 * 64 * sizeof(int32_t))};
-}
-
-LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
-    // above 128 the rows' registers leave few waves, and every 256 channels bring x to 8 bits again (256 -> 4096: 20000 rows
-    // 85 us, 64 in tiles; 512 rows 7.1 and 9.2; 256 -> 1024, 20000 rows 28 and 32)
-    if (n_in <= 128 || (n_in <= 256 && (n_out <= 1024 || (uint64_t)rows * n_out <= 1u << 22))) return LinearKernel::Rows;
-    // a fragment's 16 rows; by expert 12, since some have more (128 experts of 768 -> 1024: 12 rows 36 us, 34 in tiles; 8 rows 31, 33)
-    if (n_in > 256 && rows <= (n_experts == 1 ? 16u : 12u * n_experts)) return LinearKernel::Few;
-    return LinearKernel::Tile;
-}
 bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts) {
     const LinearKernel k = linear_i8_kernel(rows, n_in, n_out, n_experts);
     return k == LinearKernel::Rows || (k == LinearKernel::Few && linear_few_quantizes(rows, n_in, n_experts));
@@ -465,15 +442,13 @@ void launch_linear_i8(const LinearArgs& a, hipStream_t s) {
         case LinearKernel::Tile: break;
     }
     if (((uint64_t)a.x | a.ld_x | (uint64_t)a.w | a.ld_w | a.n_in) % 16 == 0) {
-        // (measured: 4096 -> 4096, 512 rows: 64 x 128 22 us, 128 x 128 31, 256 x 256 50; 2048 rows: 69, 45, 53; 8192: 256, 158, 130;
-        // 128 experts of 100 rows, 768 -> 1024: 73, 49, 58)
-        const uint32_t slots = 256;   // CUs: a round of workgroups of 64 x 128 and 256 x 256, half a round of 128 x 128
-        const uint64_t t128 = tiles_likely(a, 128, 128), t256 = tiles_likely(a, 256, 256);
         if (a.splits > 1) linear_split(a, s);
-        else if (tiles_likely(a, 64, 64) <= slots / 2) linear_stream<64, 64, 4, 4>(a, s);
-        else if (tiles_likely(a, 64, 128) <= (a.offsets ? slots * 7 / 8 : slots)) linear_stream<64, 128, 2, 4>(a, s);
-        else if (t128 <= 2 * slots || t128 * 17 <= (t256 + slots - 1) / slots * slots * 40) linear_stream<128, 128, 2, 2>(a, s);
-        else linear_stream<256, 256, 2, 2>(a, s);
+        else switch (linear_i8_tile(a.rows, a.n_out, a.n_experts, a.offsets != nullptr)) {
+            case LinearTile::T64: linear_stream<64, 64, 4, 4>(a, s); break;
+            case LinearTile::T64x128: linear_stream<64, 128, 2, 4>(a, s); break;
+            case LinearTile::T128: linear_stream<128, 128, 2, 2>(a, s); break;
+            case LinearTile::T256: linear_stream<256, 256, 2, 2>(a, s); break;
+        }
         return;
     }
     if (a.y_dtype == DT_F16) linear<_Float16>(a, s);

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "linear_i8_rule.h"
+
 namespace sng {
 
 enum { DT_F16 = 0, DT_BF16 = 1, DT_F32 = 2, DT_I8 = 3 };   // SNG_F16 ...
@@ -73,8 +75,6 @@ struct QuantArgs {
     uint64_t ld_q;
     float* scale;            // not written for DT_I8
 };
-// Which kernel: by the sizes alone, so that the workspace's size is known before the call.
-enum class LinearKernel { Rows, Few, Tile };
 struct LinearArgs {
     const void* x;           // [rows][ld_x] of x_dtype
     uint64_t ld_x;           // elements
@@ -93,12 +93,8 @@ struct LinearArgs {
     uint32_t splits;         // above 1: linear_i8_split's answer, and its workspace
     int32_t* partial;
 };
-LinearKernel linear_i8_kernel(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts);
 // whether the kernel brings x to 8 bits itself (else x has to be DT_I8)
 bool linear_i8_quantizes(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts);
-// into how many parts the sums over n_in are split where there are few tiles, and the bytes of the parts' sums
-struct LinearSplit { uint32_t splits; uint64_t bytes; };
-LinearSplit linear_i8_split(uint32_t rows, uint32_t n_in, uint32_t n_out, uint32_t n_experts);
 void launch_quantize_rows(const QuantArgs& a, hipStream_t s);
 // rows of n >= 16 bytes at any place to rows of `padded` (a multiple of 16), zeros behind n
 void launch_pad_rows(const int8_t* w, uint64_t ld_w, uint32_t n, uint64_t rows, uint32_t padded, int8_t* to, hipStream_t s);
