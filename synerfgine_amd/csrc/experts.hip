@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
     const T* __restrict__ src = (const T*)a.src;
     T* __restrict__ dst = (T*)a.dst;
     for (uint32_t b = blockIdx.x; b * (uint64_t)rows_per_block < a.n; b += gridDim.x)
-#pragma unroll (J <= 2 ? 2 : 1)
+#pragma unroll J <= 2 ? 2 : 1
         for (uint32_t i = threadIdx.x, t0 = b * rows_per_block, rows = min(rows_per_block, a.n - t0); i < rows * pieces.count.d; i += 256) {
             const uint32_t r = pieces.count.div(i), c = pieces.start(i - r * pieces.count.d);
             const uint32_t first = (t0 + r) * a.k;
@@ -461,8 +461,10 @@ static void combine(const RowsArgs& a, hipStream_t s) {
 template <typename T>
 static void combine_by_width(const RowsArgs& a, hipStream_t s) {
     const int n = piece_bytes(sizeof(T), a.d) / sizeof(T);
-    if (n == 8) combine<T, 8>(a, s);
-    else if (n == 4) combine<T, 4>(a, s);
+    if constexpr (sizeof(T) == 2) {
+        if (n == 8) return combine<T, 8>(a, s);
+    }
+    if (n == 4) combine<T, 4>(a, s);
     else if (n == 2) combine<T, 2>(a, s);
     else combine<T, 1>(a, s);
 }
@@ -544,7 +546,9 @@ static void combine_backward(const RowsArgs& a, hipStream_t s) {
     const uint32_t pieces = (a.d + N - 1) / N;
     const auto blocks = [&](uint32_t g) { return grid_of(((uint64_t)a.n * g + 255) / 256); };
     if (pieces <= 1) expert_combine_backward_kernel<T, N, 1><<<blocks(1), 256, 0, s>>>(a);
-    else if (pieces <= 4) expert_combine_backward_kernel<T, N, 4><<<blocks(4), 256, 0, s>>>(a);
+    else if constexpr (N * sizeof(T) < 16) {   // pieces below 16 bytes: the row is shorter than two of them (one element: one)
+        if constexpr (N > 1) expert_combine_backward_kernel<T, N, 4><<<blocks(4), 256, 0, s>>>(a);
+    } else if (pieces <= 4) expert_combine_backward_kernel<T, N, 4><<<blocks(4), 256, 0, s>>>(a);
     else if (pieces <= 16) expert_combine_backward_kernel<T, N, 16><<<blocks(16), 256, 0, s>>>(a);
     else if (pieces <= 128) expert_combine_backward_kernel<T, N, 64><<<blocks(64), 256, 0, s>>>(a);
     else expert_combine_backward_kernel<T, N, 256><<<grid_of(a.n), 256, 0, s>>>(a);
@@ -553,8 +557,10 @@ static void combine_backward(const RowsArgs& a, hipStream_t s) {
 template <typename T>
 static void combine_backward_by_width(const RowsArgs& a, hipStream_t s) {
     const int n = piece_bytes(sizeof(T), a.d) / sizeof(T);
-    if (n == 8) combine_backward<T, 8>(a, s);
-    else if (n == 4) combine_backward<T, 4>(a, s);
+    if constexpr (sizeof(T) == 2) {
+        if (n == 8) return combine_backward<T, 8>(a, s);
+    }
+    if (n == 4) combine_backward<T, 4>(a, s);
     else if (n == 2) combine_backward<T, 2>(a, s);
     else combine_backward<T, 1>(a, s);
 }

@@ -154,11 +154,13 @@ static void linear_few_of(const LinearArgs& a, hipStream_t s) {
     const dim3 grid((a.n_out + 16 * CT - 1) / (16 * CT), a.offsets ? a.n_experts : 1);
     // short sums: 8 waves where they all find room, so that more rows are brought to 8 bits at a time (1024 -> 1024: 8 rows 4.2 us,
     // 5.0 with 4 waves; 16 experts of 1024 -> 2048, 4 rows each: 9.5 and 8.6)
-    if (a.n_in <= 1024 && CT > 1) linear_i8_few_kernel<DT, 4, 4, CT, ODD><<<grid, 256, lds, s>>>(a, group, stride);
-    else if (a.n_in <= 1024) linear_i8_few_kernel<DT, 8, 2, CT, ODD><<<grid, 512, lds, s>>>(a, group, stride);
+    if constexpr (CT > 1) {
+        if (a.n_in <= 1024) linear_i8_few_kernel<DT, 4, 4, CT, ODD><<<grid, 256, lds, s>>>(a, group, stride);
+        else linear_i8_few_kernel<DT, 8, 4, CT, ODD><<<grid, 512, lds, s>>>(a, group, stride);
+    } else if (a.n_in <= 1024) linear_i8_few_kernel<DT, 8, 2, 1, ODD><<<grid, 512, lds, s>>>(a, group, stride);
     // longer ones: 16 waves where every workgroup has a CU of its own (8192 -> 1024: a row 6.8 us, 7.8 with 8; 2048 -> 8192: 7.1 and 6.8)
-    else if (CT == 1 && grid.x * grid.y <= 256) linear_i8_few_kernel<DT, 16, 4, 1, ODD><<<grid, 1024, lds, s>>>(a, group, stride);
-    else linear_i8_few_kernel<DT, 8, (CT > 1 ? 4 : 8), CT, ODD><<<grid, 512, lds, s>>>(a, group, stride);
+    else if (grid.x * grid.y <= 256) linear_i8_few_kernel<DT, 16, 4, 1, ODD><<<grid, 1024, lds, s>>>(a, group, stride);
+    else linear_i8_few_kernel<DT, 8, 8, 1, ODD><<<grid, 512, lds, s>>>(a, group, stride);
 }
 
 template <int DT>
