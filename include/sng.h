@@ -185,6 +185,7 @@ int sng_expert_sort_workspace(uint32_t n, uint32_t k, uint32_t n_experts, uint64
 int sng_expert_sort(sng_ctx* ctx, const int32_t* d_experts, uint32_t n, uint32_t k, uint32_t n_experts, int32_t* d_offsets,
                     int32_t* d_order, int32_t* d_slot, void* d_workspace, uint64_t workspace_bytes, void* hip_stream);
 /* d_rows[slot] = d_x[t] for every kept choice, rows of d elements of any type; other rows of d_rows stay as they are.
+ * The plan is given whole, the rows are placed by d_slot alone: d_order must not be NULL and is not read.
  * Gradient: sng_expert_combine of the rows' gradients without weights. */
 int sng_expert_dispatch(sng_ctx* ctx, const void* d_x, int32_t dtype, uint32_t d, uint64_t ld_x, const int32_t* d_order,
                         const int32_t* d_slot, uint32_t n, uint32_t k, void* d_rows, uint64_t ld_rows, void* hip_stream);

@@ -198,7 +198,8 @@ class Testbed:
         check(self._lib.sng_expert_sort(self.ctx, d_experts, n, k, n_experts, d_offsets, d_order, d_slot, d_workspace, workspace_bytes, stream))
 
     def expert_dispatch(self, d_x, dtype, d, ld_x, d_order, d_slot, n, k, d_rows, ld_rows, stream=0):
-        """Rows of x [n][d] in the experts' order; rows of no choice stay as they are.  Any type."""
+        """Rows of x [n][d] in the experts' order; rows of no choice stay as they are.  Any type.  (Placed by the slots; the
+        order is asked for as the other half of the plan and not read.)"""
         try:
             _u32[6](dtype, d, ld_x, n, k, ld_rows)
         except struct.error as error:

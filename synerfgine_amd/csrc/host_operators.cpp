@@ -100,7 +100,7 @@ void expert_dispatch(sng_ctx* c, const void* x, int32_t dtype, uint32_t d, uint6
     OnDevice on(c);
     if (n == 0) return;
     RowsArgs a{};
-    a.src = x; a.ld_src = ld_x; a.dst = rows; a.ld_dst = ld_rows; a.order = order; a.slot = slot; a.n = n; a.k = k; a.d = d; a.dtype = dtype;
+    a.src = x; a.ld_src = ld_x; a.dst = rows; a.ld_dst = ld_rows; a.slot = slot; a.n = n; a.k = k; a.d = d; a.dtype = dtype;
     launch_expert_dispatch(a, s);
     HIPCHK(hipGetLastError());
 }

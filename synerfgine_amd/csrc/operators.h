@@ -53,7 +53,6 @@ struct RowsArgs {
     uint64_t ld_dy;
     const float* weights;    // null: ones
     float* dweights;         // backward, may be null
-    const int32_t* order;    // dispatch
     const int32_t* slot;
     uint32_t n, k, d;
     int dtype;
