@@ -24,8 +24,8 @@ F16, BF16, F32, I8 = 0, 1, 2, 3   # element types (SNG_F16 ...)
 
 
 # Numbers that do not fit their C arguments would lose their high bits in ctypes: these raise struct.error for them
-_u32 = {n: struct.Struct("=%dI" % n).pack for n in (3, 5, 6, 7, 9)}
-_u64 = struct.Struct("=Q").pack
+_u32 = {n: struct.Struct("=%dI" % n).pack for n in (3, 5, 6, 7)}
+_u32_u64 = {n: struct.Struct("=%dIQ" % n).pack for n in (3, 9)}
 
 
 def _too_large(error):
@@ -191,8 +191,7 @@ class Testbed:
         """Expert ids int32 [n][k] -> the plan: offsets [n_experts + 1], order [n * k], slot [n][k] (all int32).  Ids outside
         [0, n_experts) drop their choice; an expert's rows keep the order of their choices."""
         try:
-            _u32[3](n, k, n_experts)
-            _u64(workspace_bytes)
+            _u32_u64[3](n, k, n_experts, workspace_bytes)
         except struct.error as error:
             raise _too_large(error) from None
         check(self._lib.sng_expert_sort(self.ctx, d_experts, n, k, n_experts, d_offsets, d_order, d_slot, d_workspace, workspace_bytes, stream))
@@ -254,8 +253,7 @@ class Testbed:
         """The linear layer in 8-bit integers: y = act((q w^T) * x_scale * w_scale + bias).  x F16 / BF16 / F32 is brought to 8
         bits within the call; I8 comes with d_x_scale.  d_offsets (expert_sort's): one matrix for each expert's rows."""
         try:
-            _u32[9](x_dtype, rows, n_in, ld_x, ld_w, n_out, y_dtype, ld_y, n_experts)
-            _u64(workspace_bytes)
+            _u32_u64[9](x_dtype, rows, n_in, ld_x, ld_w, n_out, y_dtype, ld_y, n_experts, workspace_bytes)
         except struct.error as error:
             raise _too_large(error) from None
         args = _lib.sng_linear_i8_args(d_x, d_x_scale, d_w, d_w_scale, d_bias, d_offsets, d_y, d_workspace, workspace_bytes, ld_x, ld_w, ld_y, rows, n_in,
