@@ -204,8 +204,8 @@ __global__ __launch_bounds__(NW * 64) void expert_place_kernel(SortArgs a, uint3
     // a thread's experts: a run of `per`, so that one scan over the workgroup does for all of them.  Their counts are asked
     // for long before they are wanted (the first one's stay in registers).
     const uint32_t per = (e_n + NW * 64 - 1) / (NW * 64), e0 = min(e_n, threadIdx.x * per), e1 = min(e_n, e0 + per);
-    const uint32_t* __restrict__ totals = ADDS ? all : a.counts + (size_t)blocks * e_n;
-    const uint32_t* __restrict__ befores = ADDS ? before : a.counts + (size_t)blockIdx.x * e_n;
+    const uint32_t* totals = ADDS ? all : a.counts + (size_t)blocks * e_n;
+    const uint32_t* befores = ADDS ? before : a.counts + (size_t)blockIdx.x * e_n;
     uint32_t total0 = 0, before0 = 0;
     if (!ADDS && e0 < e1) {
         total0 = totals[e0];
