@@ -207,7 +207,8 @@ int sng_quantize_rows_i8(sng_ctx* ctx, const void* d_x, int32_t dtype, uint32_t 
 /* y[r][c] = act((sum_k q[r][k] w[c][k]) * w_scale[c] * x_scale[r] + bias[c]): the sum exact in 32-bit integers, the rest
  * f32, rounded once to y_dtype.  x_dtype SNG_I8: q = d_x with d_x_scale; else d_x is brought to 8 bits as above within
  * the call.  d_offsets (sng_expert_sort's) gives rows [d_offsets[e], d_offsets[e + 1]) the e-th of n_experts matrices, one
- * after the other in d_w, d_w_scale and d_bias; rows outside stay as they are in d_y.  d_offsets NULL: one matrix for all
+ * after the other in d_w, d_w_scale and d_bias (d_w may be read in whole words: the bytes that share a first or last word
+ * with it are read too, and count nothing); rows outside stay as they are in d_y.  d_offsets NULL: one matrix for all
  * rows.  n_in <= 131071. */
 typedef struct {
     const void* d_x;             /* [rows][ld_x] */
