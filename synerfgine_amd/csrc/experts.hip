@@ -2,8 +2,8 @@
 //
 // A choice i = t * k + j sends sample t to expert ids[i]; an id outside [0, E) drops the choice.  The plan is a stable
 // counting sort: offsets[e] choices lie before expert e, slot[i] is choice i's row in the sorted order, order[row] = i.
-// Everything after the sort is a gather: no kernel here adds with atomics across workgroups, so results do not depend on
-// the order in which workgroups run.
+// Behind the sort rows are scattered (dispatch, the rows' gradient: each has one source) or gathered (combine): no kernel
+// here adds with atomics across workgroups, so results do not depend on the order in which workgroups run.
 #include <algorithm>
 #include <initializer_list>
 
@@ -331,7 +331,9 @@ __device__ __forceinline__ void put_piece(void* p, const V& v) { __builtin_memcp
 
 // Each sample's row to all its places: x is read once and in order, and a row's pieces go out together.  (The other way
 // round, rows of the sorted order gathered, reads a cache line of x for each 28-byte row: 2^20 x 2 such rows 45 us, this way
-// 23.)  Bound by memory, there by the parts of lines that its writes touch: 4.1 TB/s.
+// 23, or 27 with nothing in the card's caches.)  Bound by memory, there by the parts of lines that its writes touch: 4.1 TB/s.
+// Two choices are asked for together with the pieces: 2^20 x 2 rows of 28 bytes 26.8 us, in the loop over k 27.8; 2^18 x 2 of
+// 68 bytes 20.9 and 23.4, of 252 bytes 57 and 60.
 template <typename T, int K>   // a piece's bytes; K > 0: k, whose places are asked for together with the pieces
 __global__ __launch_bounds__(256) void expert_scatter_kernel(RowsArgs a, uint32_t elem, uint32_t samples_per_block, Pieces pieces) {
     constexpr int U = 4;
@@ -376,8 +378,9 @@ template <typename T>
 static void scatter(const RowsArgs& a, uint32_t elem, hipStream_t s) {
     const Pieces pieces(a.d, sizeof(T) / elem);
     // Rows of half a line and less: one workgroup a CU, with a run of samples each, so that the parts of a line that its steps
-    // write one after the other meet in the die's cache.  (2^20 x 2 rows of 28 bytes 23 us, 27 in as many workgroups as fit; 2^18
-    // x 4 rows 11.8 and 17.0; rows of 252 bytes 37.0 and 35.8.)
+    // write one after the other meet in the die's cache.  (Nothing in the caches: 2^20 x 2 rows of 28 bytes 26.8 us, 38.1 in as many
+    // workgroups as fit; 2^18 x 4 of them 17.4 and 22.9; 2^18 x 2 rows of 64 bytes 14.4 and 15.0, of 128 bytes 23.9 and 22.1;
+    // 16384 x 2 of 4096 bytes 41.7 and 39.1.)
     const uint32_t few = a.d * elem <= 64 ? (a.n + 255) / 256 : 1, samples = std::max(std::max(1u, 1024u / pieces.count.d), few);
     const uint32_t grid = grid_of((a.n + samples - 1) / samples);
     if (a.k == 2) expert_scatter_kernel<T, 2><<<grid, 256, 0, s>>>(a, elem, samples, pieces);
@@ -397,7 +400,8 @@ void launch_expert_dispatch(const RowsArgs& a, hipStream_t s) {
 
 // y[t] = sum_j w[t,j] rows[slot[t,j]], f32 in the order of j, rounded once.  The places and weights of J choices are asked
 // for together, then their J pieces, so that a thread waits twice for J choices and not twice for each.  Bound by memory:
-// 4099 x 8 rows of 4096 bf16, 302 MB, 64 us (4.7 TB/s); 2^20 x 2 rows of 4 f16, 42 MB, 9.0 us (4.7).
+// 4099 x 8 rows of 4096 bf16, 302 MB, 64 us (4.7 TB/s); 2^20 x 2 rows of 4 f16, 42 MB, 9.0 us where the rows are in the card's
+// caches (4.7), 13.9 from memory (3.0).
 template <typename T, int N, int J>
 __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_t rows_per_block, Pieces pieces) {
     using V = vec<T, N>;
@@ -448,8 +452,9 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(RowsArgs a, uint32_
 template <typename T, int N>
 static void combine(const RowsArgs& a, hipStream_t s) {
     const Pieces pieces(a.d, N);
-    // four pieces a thread where there is work for the chip in that, and a sample's choices are one load (2^20 x 2 rows of 4 f16
-    // 9.0 us, one piece a thread 11.9; 2^18 x 4 rows 6.1 and 5.3, 2^18 x 2 rows of 128 28.2 and 27.6)
+    // four pieces a thread where there is work for the chip in that, and a sample's choices are one load (rows in the caches, as a
+    // layer that has just written them leaves them: 2^20 x 2 rows of 4 f16 9.0 us, one piece a thread 11.9; 2^18 x 4 rows 6.1 and
+    // 5.3, 2^18 x 2 rows of 128 28.2 and 27.6; from memory one piece is ahead: 13.9 and 13.2, 2^18 x 2 rows of 16 10.0 and 8.6)
     const bool four = a.k <= 2 && pieces.count.d <= 8 && (uint64_t)a.n * pieces.count.d >= 1u << 19;
     const uint32_t rows = std::max(1u, (four ? 1024u : 256u) / pieces.count.d), grid = grid_of((a.n + rows - 1) / rows);
     if (a.k == 1) expert_combine_kernel<T, N, 1><<<grid, 256, 0, s>>>(a, rows, pieces);
@@ -475,7 +480,7 @@ void launch_expert_combine(const RowsArgs& a, hipStream_t s) {
     else combine_by_width<float>(a, s);
 }
 
-// The gradient of the combine, sample by sample: G threads share one sample, so dy's row is read once for all its
+// The gradient of the combine, sample by sample: G threads share one sample, so dy's row is read once for four of its
 // choices, each row of the sorted order is read and its gradient written once, and a choice's weight gradient is one
 // reduction over the G threads (f32 sums, one per thread, then a tree).  Bound by memory: 16384 x 2 rows of 2048 f16,
 // 336 MB, 63 us (5.3 TB/s, a large copy's rate).

@@ -162,7 +162,7 @@ __device__ __forceinline__ Raw<DT, 16> load_row16(const char* __restrict__ row, 
 }
 // The same for bytes at odd places: whole words that hold them (4 and the one of the last byte, none without a byte of the
 // 16), shifted together when they are wanted.  A 16-byte load that is not aligned to words takes several times as
-// long (a row times 4097 -> 4096, 8 waves: 18 us, 10 this way, 5.6 for 4096).
+// long (a row times 4097 -> 4096: 15.2 us, 9.5 this way, 6.8 for 4096; 1025 -> 2048: 6.7 and 4.8).
 struct OddBytes { uint32_t w[5], shift; };
 __device__ __forceinline__ OddBytes load_odd16(const char* __restrict__ row, uint32_t k, uint32_t n) {
     const char* p = row + min(k, n - 16);

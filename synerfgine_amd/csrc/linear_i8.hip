@@ -265,8 +265,8 @@ __global__ __launch_bounds__(256) void linear_i8_tile_kernel(LinearArgs a) {
 // the matrix units would wait for the queue.  A lane fetches the piece of its row that belongs at its place in LDS, which
 // keeps the lanes of a fragment read on different banks.
 // Wants n_in, both strides and both addresses in multiples of 16 bytes.
-// 8192 x 4096 -> 8192: 235 us, 2.3 * 10^15 operations a second (torch's int8 product into int32: 281 us).  What bounds it is
-// the card's power: an earlier form took 290 us of random values and 203 of zeros.  By expert (16384 rows on 16, 2048 -> 4096) 177 us: row tiles that an
+// 8192 x 4096 -> 8192: 237 us, 2.3 * 10^15 operations a second (torch's int8 product into int32: 281 us).  What bounds it is
+// the card's power: an earlier form took 290 us of random values and 203 of zeros.  By expert (16384 rows on 16, 2048 -> 4096) 179 us: row tiles that an
 // expert fills in part (an eighth of the work) and 4.5 rounds of tiles that take the time of 5.
 __device__ const int8_t zeros16[16] __attribute__((aligned(16))) = {};
 

@@ -3,8 +3,8 @@
 
 namespace sng {
 
-// Bound by reading the weights once (16 experts of 1024 -> 2048, 48 rows: 33.5 MB, 9.5 us, 3.5 TB/s), and for the smallest by
-// the chain of waits (one row, 4096 -> 4096: 7 us, 5.3 where the weights are in the card's caches).  A workgroup takes 16 CT channels of one
+// Bound by reading the weights once (16 experts of 1024 -> 2048, 48 rows: 33.5 MB, 10.6 us, 3.2 TB/s), and for the smallest by
+// the chain of waits (one row, 4096 -> 4096: 6.2 us, 5.2 where the weights are in the card's caches).  A workgroup takes 16 CT channels of one
 // matrix and splits n_in over its NW waves, so that a whole chip of waves is loading also for one row; each wave's sums meet
 // in LDS.  x (up to 16 rows at a time) in floating point is brought to 8 bits on the way, by all waves together, into LDS,
 // where the fragments are read from: with few rows most lanes of a fragment would have none to work on.  Every workgroup does
@@ -12,9 +12,9 @@ namespace sng {
 // loads come back in their order, and the weights have the time that the rows' way to 8 bits takes.
 //
 // A call runs every instruction about once, out of a cold instruction cache: what is repeated is a loop, and the weights of
-// a row's end are taken as load_row16 gives them.  (4097 -> 4096, one row, 8 waves: 18 us; 20.5 us with code between
-// the matrix instructions that moves them to their places, each jump over it a miss.  ODD: weights at odd places, 10 us;
-// with 16 waves 8.7.)
+// a row's end are taken as load_row16 gives them.  (4097 -> 4096, one row, 8 waves, before ODD: 18 us; 20.5 us with code between
+// the matrix instructions that moves them to their places, each jump over it a miss.  ODD: weights at odd places, 9.2 us
+// with 16 waves.)  The figures of the rules below are of calls on the same buffers again, the weights in the card's caches.
 constexpr uint32_t FEW_LDS = 60 * 1024;   // for x's rows
 static uint32_t few_stride(uint32_t n_in) { return (n_in + 63) / 64 * 64 + 16; }   // (+ 16: the rows of a fragment read lie on different banks)
 

@@ -10,7 +10,7 @@ namespace sng {
 // ds_read_b128 a fragment, no bank conflicts), staged once for the workgroup's rows, which belong to one expert.
 // x of type DT; KC fragments of 64 a row; NB blocks of 64 channels.  YT: y's type, or -1: any, at more registers and so fewer
 // waves; -2: any, and n_in below 16.  What hides the memory's latency here is waves, in small workgroups.  2^20 x 64 -> 64
-// f16: 268 MB, 52 us (5.1 TB/s, a large copy's rate); by expert, 2^19 rows on 512 experts, 32 -> 64: 29.5 us (3.4 TB/s: 32
+// f16: 268 MB, 53 us (5.1 TB/s, a large copy's rate); by expert, 2^19 rows on 512 experts, 32 -> 64: 31.5 us (3.2 TB/s: 32
 // values fill half of the matrix instruction).
 template <int DT, int YT, int KC, int NB>
 __global__ __launch_bounds__(256) void linear_i8_rows_kernel(LinearArgs a, uint32_t shift) {

@@ -1,5 +1,5 @@
 // linear_i8_rule.h -- which kernel of the 8-bit linear layer (linear_i8.hip) a call takes, by its sizes alone, so that the
-// workspace's size is known before the call.  Plain host code.
+// workspace's size is known before the call.  Plain host code.  Figures: calls on the same buffers again.
 #pragma once
 #include <algorithm>
 #include <stdint.h>
