@@ -4,7 +4,7 @@
 namespace sng {
 
 // Bound by reading the weights once (16 experts of 1024 -> 2048, 48 rows: 33.5 MB, 10.6 us, 3.2 TB/s), and for the smallest by
-// the chain of waits (one row, 4096 -> 4096: 6.2 us, 5.2 where the weights are in the card's caches).  A workgroup takes 16 CT channels of one
+// the chain of waits (one row, 4096 -> 4096: 6.8 us from memory, 5.2 from the dies' caches).  A workgroup takes 16 CT channels of one
 // matrix and splits n_in over its NW waves, so that a whole chip of waves is loading also for one row; each wave's sums meet
 // in LDS.  x (up to 16 rows at a time) in floating point is brought to 8 bits on the way, by all waves together, into LDS,
 // where the fragments are read from: with few rows most lanes of a fragment would have none to work on.  Every workgroup does
